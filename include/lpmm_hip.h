@@ -820,6 +820,85 @@ enum {
 int lpmm_stream_probe(int kind, float *a, const float *b, uint8_t *codes0, uint8_t *codes1, float *scale0,
                       float *scale1, int64_t n, int64_t lds_bytes, void *stream);
 
+/* ---------------------------------------------------------------------------------------
+ * (e) Terms of a training loss with their gradients.  No counterpart in the reference, whose users
+ *     take them from elsewhere: they stand at the other end of the training step whose end the
+ *     optimizer steps above are.
+ * ------------------------------------------------------------------------------------- */
+enum { LPMM_TYPE_F32 = 0, LPMM_TYPE_F16 = 1, LPMM_TYPE_BF16 = 2,
+       LPMM_TYPE_CODES = 3 /* teacher values only: codes in the packed layout of lpmm_quant_group (4 bits) and lpmm_quant_group_bits */ };
+enum { LPMM_REDUCE_NONE = 0, LPMM_REDUCE_SUM = 1, LPMM_REDUCE_MEAN = 2 };
+/* Most teacher entries a row may have. */
+#define LPMM_DISTILL_MOST 1024
+
+/* Distillation from a teacher's top logits, with the cross entropy of a label from the same pass.  HOST memory, read during the call.
+ * Row n has logits x[vocab], topk teacher entries (value t_k, id i_k) and a label y.  With T = temperature, q = softmax(x / T) and
+ * p = softmax(t / T) over the entries whose id is not negative:
+ *   kd_n   = T^2 sum_k p_k (log p_k - log q[i_k])      0 for a row without entries, or with values of -infinity only
+ *   ce_n   = logsumexp(x) - x[y]                        0 without labels
+ *   loss_n = teacher_weight kd_n + label_weight ce_n
+ * A row whose label is ignore_index takes no part: its loss and gradient are 0 whatever it holds, and the mean does not count it.
+ * The mean of no rows is 0.  An id of vocab or more, a label outside [0, vocab) that is not ignore_index, a value of NaN or
+ * +infinity make the row's loss and gradient NaN.  An id that occurs several times counts with the sum of its probabilities. */
+typedef struct lpmm_distill_call {
+    const void *logits;         /* row n at element (n / inner) * outer_stride + (n % inner) * inner_stride, its values side by side */
+    const void *teacher;        /* [rows][topk] values of teacher_type */
+    const float *teacher_scale; /* codes: one scale per teacher_group values of the flattened array */
+    const float *teacher_map;   /* codes: 2^teacher_bits entries */
+    const void *ids;            /* [rows][topk] int32 or int64 (id_bits) */
+    const int64_t *labels;      /* [rows], or NULL */
+    float *row_loss;            /* [rows]: the loss of each row (written in every reduction) */
+    float *row_stats;           /* [rows][4], 16-byte aligned: what the gradient call needs of each row; NULL: not kept */
+    float *loss;                /* [1]: the reduced loss; NULL with LPMM_REDUCE_NONE */
+    float *share;               /* [1]: work of the mean with labels, kept for the gradient call: 1 / rows that count */
+    void *grad;                 /* [rows][vocab] of `type`: the reduced loss's gradient, from the same pass; NULL: not wanted */
+    int64_t rows, vocab, topk;  /* vocab: 1 .. 2^31 - 1; topk: 0 .. LPMM_DISTILL_MOST */
+    int64_t inner, outer_stride, inner_stride;
+    int64_t teacher_group;      /* codes: values per scale, 1 or more */
+    int64_t ignore_index;
+    float temperature;          /* 1/1024 .. 1024 */
+    float teacher_weight, label_weight;
+    int32_t type, teacher_type, id_bits, reduction;
+    int32_t teacher_bits;       /* codes: 4 (two a byte) or 5 .. 8 (a byte each) */
+} lpmm_distill_call;
+
+/* loss, row_loss, row_stats and grad of the call.  grad with LPMM_REDUCE_NONE is an LPMM_ERR_ARG. */
+int lpmm_distill_loss(const lpmm_distill_call *call, void *stream);
+
+/* The gradient of a loss that lpmm_distill_loss has computed: call as it was there, its row_stats and share as that call left them,
+ * grad the array to write.  grad_loss: device memory, the gradient of the loss, one value or (LPMM_REDUCE_NONE) one per row,
+ * grad_loss_stride elements apart.  made != 0: grad holds the gradient for *grad_loss == 1 already (lpmm_distill_loss wrote
+ * it); it is written again only where *grad_loss is another value. */
+int lpmm_distill_loss_grad(const lpmm_distill_call *call, const float *grad_loss, int64_t grad_loss_stride, int made, void *stream);
+
+/* Balance of a router's experts, in groups of tokens (one group: a batch; more: a sequence or layer each).  HOST memory, read during
+ * the call.  Token n of a group has router logits r_n[experts], p_n = softmax(r_n), and `picks` ids of the experts it goes to; tokens
+ * whose mask is 0 take no part.  With T the tokens of the group that do and c_e the picks of expert e among theirs:
+ *   loss_g = weight * experts * sum_e c_e / (T picks) * (sum_n p_ne / T)  +  z_weight * sum_n logsumexp(r_n)^2 / T      0 for T = 0
+ *   loss   = sum_g loss_g / groups
+ * The counts are constants to the gradient.  A negative id is no pick; an id of `experts` or more makes the loss and its
+ * gradient NaN.  The same id twice in a row counts twice. */
+typedef struct lpmm_balance_call {
+    const void *logits;         /* token n of group g at element g * outer_stride + n * inner_stride, its values side by side */
+    const void *ids;            /* [groups][tokens][picks] int32 or int64 (id_bits); not read by the gradient call */
+    const uint8_t *mask;        /* [groups][tokens], 0 or not; NULL: every token counts */
+    float *loss;                /* [1] */
+    int64_t *counts;            /* [groups][experts] */
+    float *factors;             /* [groups][experts + 2]: what the gradient call needs */
+    void *work;                 /* lpmm_balance_work_bytes, 8-byte aligned; free again when the call's kernels have run */
+    void *grad;                 /* gradient call only: [groups][tokens][experts] of `type` */
+    int64_t groups, tokens, experts, picks; /* experts: 1 .. LPMM_BALANCE_MOST; picks: 0 .. experts; tokens * picks below 2^31 */
+    int64_t outer_stride, inner_stride;
+    float weight, z_weight;
+    int32_t type, id_bits;
+} lpmm_balance_call;
+#define LPMM_BALANCE_MOST 1024
+
+int64_t lpmm_balance_work_bytes(int64_t groups, int64_t tokens, int64_t experts);
+int lpmm_balance_loss(const lpmm_balance_call *call, void *stream);
+/* grad of the call for *grad_loss (device memory), factors as lpmm_balance_loss left them. */
+int lpmm_balance_loss_grad(const lpmm_balance_call *call, const float *grad_loss, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

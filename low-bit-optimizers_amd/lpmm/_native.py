@@ -4,6 +4,7 @@ There is no fallback: if the library is missing or a call fails, a RuntimeError 
 """
 import ctypes
 import os
+import struct
 import warnings
 
 import numpy as np
@@ -89,6 +90,11 @@ PROTOTYPES = {
     "lpmm_factored_fp32_step_multi": (_int, [_vp, _i64, _int, _vp, _i64, _int, _vp] + [_d] * 5 + [_vp]),
     "lpmm_sgd4bit_fp32_step_multi": (_int, [_vp, _i64, _vp, _i64, _vp] + [_d] * 4 + [_int] * 2 + [_vp]),
     "lpmm_sgd_fp32_step_multi": (_int, [_vp, _i64] + [_d] * 4 + [_int, _int, _vp]),
+    "lpmm_distill_loss": (_int, [_vp, _vp]),
+    "lpmm_distill_loss_grad": (_int, [_vp, _vp, _i64, _int, _vp]),
+    "lpmm_balance_work_bytes": (_i64, [_i64] * 3),
+    "lpmm_balance_loss": (_int, [_vp, _vp]),
+    "lpmm_balance_loss_grad": (_int, [_vp, _vp, _vp]),
     "lpmm_stream_probe": (_int, [_int] + [_vp] * 6 + [_i64, _i64, _vp]),
     "lpmm_selftest_encoders": (_int, [_vp, _vp]),
     "lpmm_selftest_bucket_encoder": (_int, [_vp, _int, _vp, _vp]),
@@ -134,6 +140,14 @@ SGD_FP32_TENSOR = np.dtype([("p", "<u8"), ("g", "<u8"), ("buf", "<u8"), ("n", "<
                             ("reserved", "<i4")])
 ADAMW_FP32_TENSOR = np.dtype([("p", "<u8"), ("g", "<u8"), ("m", "<u8"), ("v", "<u8"), ("n", "<i8"),
                               ("step", "<f4"), ("reserved", "<f4")])
+
+# the calls of the training-loss terms (lpmm_distill_call, lpmm_balance_call), one to a record
+DISTILL_CALL = struct.Struct("<11Q8q3f5i")
+BALANCE_CALL = struct.Struct("<8Q6q2f2i")
+TYPE_F32, TYPE_F16, TYPE_BF16, TYPE_CODES = range(4)
+REDUCE_NONE, REDUCE_SUM, REDUCE_MEAN = range(3)
+DISTILL_MOST = 1024  # teacher entries of a row (LPMM_DISTILL_MOST)
+BALANCE_MOST = 1024  # experts of a router (LPMM_BALANCE_MOST)
 
 _lib = None
 

@@ -424,3 +424,7 @@ def vectorwise_dequant(qx, denormalized=True, **kwargs):
 
 def numel(shape):
     return math.prod(shape)
+
+
+# terms of a training loss (lpmm/losses.py); at the end: a stored teacher is read with the helpers above
+from .losses import balance_loss, distill_loss  # noqa: E402, F401
