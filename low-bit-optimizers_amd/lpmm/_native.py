@@ -4,7 +4,6 @@ There is no fallback: if the library is missing or a call fails, a RuntimeError 
 """
 import ctypes
 import os
-import struct
 import warnings
 
 import numpy as np
@@ -141,14 +140,6 @@ SGD_FP32_TENSOR = np.dtype([("p", "<u8"), ("g", "<u8"), ("buf", "<u8"), ("n", "<
 ADAMW_FP32_TENSOR = np.dtype([("p", "<u8"), ("g", "<u8"), ("m", "<u8"), ("v", "<u8"), ("n", "<i8"),
                               ("step", "<f4"), ("reserved", "<f4")])
 
-# the calls of the training-loss terms (lpmm_distill_call, lpmm_balance_call), one to a record
-DISTILL_CALL = struct.Struct("<11Q8q3f5i")
-BALANCE_CALL = struct.Struct("<8Q6q2f2i")
-TYPE_F32, TYPE_F16, TYPE_BF16, TYPE_CODES = range(4)
-REDUCE_NONE, REDUCE_SUM, REDUCE_MEAN = range(3)
-DISTILL_MOST = 1024  # teacher entries of a row (LPMM_DISTILL_MOST)
-BALANCE_MOST = 1024  # experts of a router (LPMM_BALANCE_MOST)
-
 _lib = None
 
 
@@ -201,6 +192,24 @@ def walk():
             module = _NoWalk()
         _walk = module
     return _walk
+
+
+_losses = None
+
+
+def losses():
+    """The host side of the training-loss terms (csrc/losses.cpp): an extension module, built against one version of torch and of
+    Python.  Nothing stands in for it."""
+    global _losses
+    if _losses is None:
+        lib()
+        try:
+            from . import _losses as module
+        except ImportError as e:
+            raise RuntimeError(f"lpmm: the extension module lpmm/_losses.so does not load ({e}). Build it with "
+                               "`make -C low-bit-optimizers_amd/csrc`.") from e
+        _losses = module
+    return _losses
 
 
 _factored_workspace = None

@@ -3,8 +3,15 @@
 Every function returns values and, beside each, a bound on what 32-bit arithmetic may add to it.  U = 2^-24 is half a step of
 float32 relative to the value; the bounds count roundings along the longest path and are not fitted to any result."""
 import math
+import struct
 
 import torch
+
+# the library's calls (lpmm_distill_call, lpmm_balance_call), and its names for types and reductions
+DISTILL_CALL = struct.Struct("<11Q8q3f5i")
+BALANCE_CALL = struct.Struct("<8Q6q2f2i")
+TYPE_F32, TYPE_F16, TYPE_BF16, TYPE_CODES = range(4)
+REDUCE_NONE, REDUCE_SUM, REDUCE_MEAN = range(3)
 
 U = 2.0 ** -24
 TINY = 2.0 ** -126  # an exponential below the smallest normal float32 is 0, in the kernels and on the hardware: an absolute error of at most this

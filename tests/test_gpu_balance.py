@@ -216,8 +216,8 @@ def test_nothing_is_written_past_the_tokens():
     sizes = ((1, torch.float32), (39, torch.int64), (45, torch.float32), (lib.lpmm_balance_work_bytes(3, 67, 13), torch.uint8), (3 * 67 * 13, torch.bfloat16))
     room = [torch.full((n + 2 * pad,), 7, dtype=d, device="cuda") for n, d in sizes]
     loss, counts, factors, work, grad = (a[pad:].data_ptr() for a in room)
-    record = _native.BALANCE_CALL.pack(r.data_ptr(), ids.data_ptr(), mask.data_ptr(), loss, counts, factors, work, grad, 3, 67, 13, 2, 67 * 13, 13,
-                                       0.5, 0.1, _native.TYPE_BF16, 64)
+    record = ref.BALANCE_CALL.pack(r.data_ptr(), ids.data_ptr(), mask.data_ptr(), loss, counts, factors, work, grad, 3, 67, 13, 2, 67 * 13, 13,
+                                       0.5, 0.1, ref.TYPE_BF16, 64)
     one = torch.ones(1, device="cuda")
     assert lib.lpmm_balance_loss(record, _native.current_stream(0)) == 0
     assert lib.lpmm_balance_loss_grad(record, one.data_ptr(), _native.current_stream(0)) == 0

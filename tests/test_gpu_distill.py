@@ -311,7 +311,7 @@ def test_several_passes_over_one_graph():
     with pytest.raises(RuntimeError):
         torch.autograd.grad(loss, leaf)
     loss = F.distill_loss(leaf, t.cuda(), ids.cuda())
-    with pytest.raises(RuntimeError, match="once_differentiable|differentiate twice|does not require grad"):
+    with pytest.raises(RuntimeError, match="differentiate twice"):
         g = torch.autograd.grad(loss, leaf, create_graph=True)[0]
         torch.autograd.grad(g.float().sum(), leaf)
     with torch.no_grad():
@@ -398,8 +398,8 @@ def test_nothing_is_written_past_the_rows():
     room = [torch.full((n + 2 * pad,), 7.0, dtype=d, device="cuda") for n, d in ((3 * 1003, torch.bfloat16), (3, torch.float32), (12, torch.float32),
                                                                                 (1, torch.float32), (1, torch.float32))]
     grad, row_loss, stats, loss, share = (r[pad:].data_ptr() for r in room)
-    record = _native.DISTILL_CALL.pack(x.data_ptr(), t.data_ptr(), 0, 0, ids.data_ptr(), y.data_ptr(), row_loss, stats, loss, share, grad, 3, 1003, 6,
-                                       3, 0, 1003, 1, -100, 2.0, 1.0, 0.5, _native.TYPE_BF16, _native.TYPE_F32, 64, _native.REDUCE_MEAN, 8)
+    record = ref.DISTILL_CALL.pack(x.data_ptr(), t.data_ptr(), 0, 0, ids.data_ptr(), y.data_ptr(), row_loss, stats, loss, share, grad, 3, 1003, 6,
+                                       3, 0, 1003, 1, -100, 2.0, 1.0, 0.5, ref.TYPE_BF16, ref.TYPE_F32, 64, ref.REDUCE_MEAN, 8)
     lib = _native.lib()
     assert lib.lpmm_distill_loss(record, _native.current_stream(0)) == 0
     one = torch.tensor(3.0, device="cuda")

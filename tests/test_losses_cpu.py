@@ -118,7 +118,7 @@ def _distill_record(**change):
     assert list(v) == DISTILL
     for k, to in change.items():
         v[k] = at + to if isinstance(to, int) and k in DISTILL[:11] and to else to
-    return keep, _native.DISTILL_CALL.pack(*v.values())
+    return keep, ref.DISTILL_CALL.pack(*v.values())
 
 
 @pytest.mark.parametrize("status,change", [
@@ -165,7 +165,7 @@ def _balance_record(**change):
     assert list(v) == BALANCE
     for k, to in change.items():
         v[k] = at + to if k in BALANCE[:8] and to else to
-    return keep, _native.BALANCE_CALL.pack(*v.values())
+    return keep, ref.BALANCE_CALL.pack(*v.values())
 
 
 @pytest.mark.parametrize("status,change,grad", [
@@ -192,26 +192,27 @@ def test_balance_argument_errors_without_gpu(status, change, grad):
 def test_records_match_the_header():
     from lpmm import _native
 
-    assert _native.DISTILL_CALL.size == 184 and _native.BALANCE_CALL.size == 128
+    assert _native.losses().abi_version == _native.ABI_VERSION
+    assert ref.DISTILL_CALL.size == 184 and ref.BALANCE_CALL.size == 128
     assert _native.lib().lpmm_distill_loss(None, None) == NULL and _native.lib().lpmm_balance_loss(None, None) == NULL
     assert _native.lib().lpmm_balance_work_bytes(0, 5, 8) == 0 and _native.lib().lpmm_balance_work_bytes(3, 5, 8) > 0
 
 
 def test_views_of_rows_keep_their_strides():
-    from lpmm.losses import _row_strides
+    from lpmm import _native
 
+    row_strides = _native.losses().row_strides
     t = torch.zeros(4, 6, 8)
     for view, want in [(t, (24, 0, 8)), (t[:, :-1], (5, 48, 8)), (t[:, 1:, :5], (5, 48, 8)), (t[:, 0], (4, 0, 48)), (t[0, 0], (1, 0, 0)),
                        (t.transpose(0, 1), (4, 8, 48)), (t[1:2, :3], (3, 0, 8)), (t[:1].expand(3, 6, 8), (6, 0, 8))]:
-        same, *got = _row_strides(view)
-        assert tuple(got) == want and same.data_ptr() == view.data_ptr()
-        inner, outer, step = got
+        inner, outer, step = got = row_strides(view)
+        assert got == want
         index = torch.arange(t.numel()).view(t.shape).as_strided(view.shape, view.stride(), view.storage_offset())
         rows = index[..., 0].reshape(-1)
         assert [view.storage_offset() + n // inner * outer + n % inner * step for n in range(rows.numel())] == rows.tolist()
+    assert row_strides(torch.zeros(3, 0, 8)) == (1, 0, 0) and row_strides(torch.zeros(5, 1)) == (5, 0, 1)
     for copied in (torch.zeros(2, 3, 4, 8).permute(2, 1, 0, 3), torch.zeros(8, 4).t()):
-        same, inner, outer, step = _row_strides(copied)
-        assert same.is_contiguous() and (inner, outer, step) == (same.numel() // same.shape[-1], 0, same.shape[-1])
+        assert row_strides(copied) is None
 
 
 @pytest.mark.parametrize("temperature,wt,wl", [(1.0, 1.0, 0.0), (2.0, 0.5, 0.5), (0.5, 0.0, 1.0)])
