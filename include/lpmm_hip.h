@@ -852,7 +852,7 @@ typedef struct lpmm_distill_call {
     float *loss;                /* [1]: the reduced loss; NULL with LPMM_REDUCE_NONE */
     float *share;               /* [1]: work of the mean with labels, kept for the gradient call: 1 / rows that count */
     void *grad;                 /* [rows][vocab] of `type`: the reduced loss's gradient, from the same pass; NULL: not wanted */
-    int64_t rows, vocab, topk;  /* vocab: 1 .. 2^31 - 1; topk: 0 .. LPMM_DISTILL_MOST */
+    int64_t rows, vocab, topk;  /* rows: 0 .. 2^31 - 1; vocab: 1 .. 2^31 - 1; topk: 0 .. LPMM_DISTILL_MOST */
     int64_t inner, outer_stride, inner_stride;
     int64_t teacher_group;      /* codes: values per scale, 1 or more */
     int64_t ignore_index;
