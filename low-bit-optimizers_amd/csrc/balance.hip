@@ -47,14 +47,14 @@ Split split(int64_t groups, int64_t tokens)
     return {parts, (tokens + parts - 1) / parts};
 }
 
-__device__ __forceinline__ float lanes_max(float v, int lanes)
+__device__ __forceinline__ float spread_max(float v, int lanes)
 {
     for (int o = lanes >> 1; o > 0; o >>= 1)
         v = fmaxf(v, __shfl_xor(v, o, kWave));
     return v;
 }
 
-__device__ __forceinline__ float lanes_sum(float v, int lanes)
+__device__ __forceinline__ float spread_sum(float v, int lanes)
 {
     for (int o = lanes >> 1; o > 0; o >>= 1)
         v += __shfl_xor(v, o, kWave);
@@ -86,14 +86,14 @@ __device__ __forceinline__ float softmax(float (&v)[RUN], int lanes)
 #pragma unroll
     for (int j = 1; j < RUN; ++j)
         m = fmaxf(m, v[j]);
-    m = lanes_max(m, lanes);
+    m = spread_max(m, lanes);
     float s = 0.0f;
 #pragma unroll
     for (int j = 0; j < RUN; ++j) {
         v[j] = exp2_fast((v[j] - m) * kLog2e);
         s += v[j];
     }
-    s = lanes_sum(s, lanes);
+    s = spread_sum(s, lanes);
     const float inv = 1.0f / s;
 #pragma unroll
     for (int j = 0; j < RUN; ++j)
@@ -254,7 +254,7 @@ __global__ __launch_bounds__(kBalThreads) void balance_grad_kernel(Balance a)
 #pragma unroll
         for (int j = 0; j < RUN; ++j)
             dot += f[j] * v[j];
-        dot = lanes_sum(dot, a.lanes);
+        dot = spread_sum(dot, a.lanes);
         if (n >= end)
             continue;
         typename T::Raw out[RUN];

@@ -14,12 +14,15 @@
 namespace lpmm {
 namespace {
 
+constexpr int64_t kLastLevel = (int64_t)256 << 20;  // bytes of the memory-side cache
+
 struct Distill {
     lpmm_distill_call c;
     const float *grad_loss;  // the gradient call: not NULL
     int64_t grad_loss_stride;
     int made;        // the gradient call: grad holds what belongs to grad_loss == 1
     int with_label;  // labels that have a weight
+    int far;         // the logits are more than the last-level cache holds
     float each;      // weight of a row in the reduced loss where no `share` says it
 };
 
@@ -48,28 +51,73 @@ struct Shift {
     __device__ __forceinline__ float of_value(float x) const { return one_step() ? fmaf(x, c, -m) : (x - max) * c; }
 };
 
+// Of the teacher's exponentials and of the label's: both in one step or neither, and the square's exponent twice the other's.
+template <typename T, int KIND>
+__device__ __forceinline__ void shifts(float max, float c, Shift &t, Shift &one)
+{
+    t = Shift::of<T>(max, c);
+    one = KIND == kTwo ? Shift::of<T>(max, kLog2e) : KIND == kSquare ? Shift{max, kLog2e, 2.0f * t.m} : t;
+    if (KIND == kTwo && !(t.one_step() && one.one_step()))
+        t.m = one.m = NAN;
+}
+
 template <typename T>
 __device__ __forceinline__ const typename T::Raw *row_of(const lpmm_distill_call &c, int64_t row)
 {
     return static_cast<const typename T::Raw *>(c.logits) + (row / c.inner) * c.outer_stride + (row % c.inner) * c.inner_stride;
 }
 
-__device__ __forceinline__ int64_t id_of(const lpmm_distill_call &c, int64_t at)
+// One entry of the teacher, as the thread that has it keeps it.  What is loaded stays as it is stored until it is used: whoever converts
+// waits, and the row's loads have to be on their way by then.
+struct Entry {
+    int64_t id;         // -1: none
+    uint32_t value, x;  // the teacher's value and the student's logit, as stored
+    float scale;        // of a value in codes
+    float t;
+
+    __device__ __forceinline__ void load(const lpmm_distill_call &c, int64_t at)
+    {
+        if (c.id_bits == 64)
+            id = static_cast<const int64_t *>(c.ids)[at];
+        else
+            id = static_cast<const int32_t *>(c.ids)[at];
+        if (c.teacher_type == LPMM_TYPE_F32) {
+            value = static_cast<const uint32_t *>(c.teacher)[at];
+        } else if (c.teacher_type != LPMM_TYPE_CODES) {
+            value = static_cast<const uint16_t *>(c.teacher)[at];
+        } else {
+            value = static_cast<const uint8_t *>(c.teacher)[c.teacher_bits == 4 ? at >> 1 : at];
+            scale = c.teacher_scale[at / c.teacher_group];
+        }
+    }
+    __device__ __forceinline__ float value_of(const lpmm_distill_call &c, int64_t at) const
+    {
+        switch (c.teacher_type) {
+        case LPMM_TYPE_F32: return __uint_as_float(value);
+        case LPMM_TYPE_BF16: return __uint_as_float(value << 16);
+        case LPMM_TYPE_F16: return (float)__builtin_bit_cast(_Float16, (uint16_t)value);
+        default: return c.teacher_map[(c.teacher_bits == 4 ? value >> (4 * (at & 1)) : value) & ((1u << c.teacher_bits) - 1u)] * scale;
+        }
+    }
+};
+
+// A logit as it is stored.
+template <typename T>
+__device__ __forceinline__ uint32_t load_bits(const typename T::Raw *p)
 {
-    return c.id_bits == 64 ? static_cast<const int64_t *>(c.ids)[at] : static_cast<const int32_t *>(c.ids)[at];
+    if constexpr (T::kRun == 8)
+        return *reinterpret_cast<const uint16_t *>(p);
+    else
+        return *reinterpret_cast<const uint32_t *>(p);
 }
 
-__device__ __forceinline__ float teacher_of(const lpmm_distill_call &c, int64_t at)
+template <typename T>
+__device__ __forceinline__ float from_bits(uint32_t bits)
 {
-    switch (c.teacher_type) {
-    case LPMM_TYPE_F32: return static_cast<const float *>(c.teacher)[at];
-    case LPMM_TYPE_F16: return F16::get(static_cast<const F16::Raw *>(c.teacher)[at]);
-    case LPMM_TYPE_BF16: return BF16::get(static_cast<const BF16::Raw *>(c.teacher)[at]);
-    default: break;
-    }
-    const uint8_t *codes = static_cast<const uint8_t *>(c.teacher);
-    const uint32_t byte = c.teacher_bits == 4 ? codes[at >> 1] >> (4 * (at & 1)) : codes[at];
-    return c.teacher_map[byte & ((1u << c.teacher_bits) - 1u)] * c.teacher_scale[at / c.teacher_group];
+    if constexpr (T::kRun == 8)
+        return T::get(__builtin_bit_cast(typename T::Raw, (uint16_t)bits));
+    else
+        return __uint_as_float(bits);
 }
 
 // The largest of three; without the two instructions that the library's maximum spends on quieting NaN, which are ignored here too.
@@ -136,251 +184,360 @@ __device__ __forceinline__ u32x4 run_grad(u32x4 r, const Shift &t, const Shift &
     return T::pack(v);
 }
 
-// What the first wave finds out about a row's entries, in shared memory.
-struct Teacher {
-    float log_total, top;
-    int some, bad;
+// What an entry takes off at its id, where others may have the same id: the first of them takes off the parts of all, in their order.  ids and
+// part: of the row's entries, the label last; whole fours, the rest -1.  False: another entry is the first.
+__device__ __forceinline__ bool takes_off(const int *ids, const float *part, int entries, int k, float &off)
+{
+    const int id = ids[k];
+    int same = 0;
+    for (int j = 0; j < entries; j += 4) {
+        const int4 four = *reinterpret_cast<const int4 *>(ids + j);
+        same += (four.x == id) + (four.y == id) + (four.z == id) + (four.w == id);
+    }
+    off = part[k];
+    if (same > 1) {
+        for (int j = 0; j < k; ++j)
+            if (ids[j] == id)
+                return false;
+        for (int j = k + 1; j < entries; ++j)
+            if (ids[j] == id)
+                off += part[j];
+    }
+    return true;
+}
+
+// A row's values in runs of 16 bytes that start at aligned addresses of the array that matters, and up to 2 (kRun - 1) single ones at its
+// ends, one to a thread: thread i < head takes value i, thread kRun + i value end + i.
+struct Cut {
+    uint32_t head, end, vocab;  // runs: [head, end)
+    template <typename T>
+    static __device__ __forceinline__ Cut of(const void *aligned, uint32_t vocab)
+    {
+        uint32_t head = (uint32_t)(-reinterpret_cast<uintptr_t>(aligned) & 15u) / sizeof(typename T::Raw);
+        head = head < vocab ? head : vocab;
+        return {head, head + (vocab - head) / T::kRun * T::kRun, vocab};
+    }
+    // the single value of a thread, or vocab
+    template <typename T>
+    __device__ __forceinline__ uint32_t single() const
+    {
+        const uint32_t tid = threadIdx.x;
+        if (tid < head)
+            return tid;
+        return tid >= T::kRun && tid - T::kRun < vocab - end ? end + tid - T::kRun : vocab;
+    }
 };
 
-// The entries' ids (-1: empty) and probabilities; `value` keeps t.  One wave, which alone uses `value` again.
-__device__ __forceinline__ void read_teacher(const Distill &a, int64_t row, int64_t label, int *ids, float *part, float *value, Teacher *out)
+// The sums of a row as one thread, one wave or the workgroup has them: relative to `max`.
+struct Sums {
+    float max, sum, sum1;
+};
+
+template <int KIND, bool ONE_STEP>
+__device__ __forceinline__ float from_to(float from, float to, float c)
 {
-    const lpmm_distill_call &c = a.c;
-    const int lane = threadIdx.x, topk = (int)c.topk;
-    bool wrong = c.labels && (label < 0 || label >= c.vocab);
-    float top = -INFINITY;
-    for (int k = lane; k < topk; k += kWave) {
-        const int64_t at = row * topk + k, id = id_of(c, at);
-        const float t = id < 0 ? -INFINITY : teacher_of(c, at);
-        wrong |= id >= c.vocab || !(t < INFINITY);
-        top = fmaxf(top, t);
-        ids[k] = id < 0 || id >= c.vocab ? -1 : (int)id;
-        value[k] = t;
-    }
-    top = wave_max(top);
-    const bool some = top > -INFINITY;
-    const float inv_t = 1.0f / c.temperature;
-    float total = 0.0f;
-    for (int k = lane; k < topk; k += kWave) {
-        const float p = some && ids[k] >= 0 ? expf((value[k] - top) * inv_t) : 0.0f;
-        part[k] = p;
-        total += p;
-    }
-    total = wave_sum(total);
-    const float inv = some ? 1.0f / total : 0.0f;
-    for (int k = lane; k < topk; k += kWave)
-        part[k] *= inv;
-    const int round = (topk + 1 + 3) & ~3;  // the label's place, and what fills the last four
-    if (lane < round - topk) {
-        ids[topk + lane] = lane == 0 && a.with_label && label >= 0 && label < c.vocab ? (int)label : -1;
-        part[topk + lane] = 0.0f;
-    }
-    const bool bad = __any(wrong);
-    if (lane == 0)
-        *out = {some ? logf(total) : 0.0f, top, some, bad};
+    return ONE_STEP ? exp2_fast(from * c - to * c) : exp2_fast((from - to) * c);
 }
 
-// The row's loss; one wave, once the sums are known.
-template <typename T>
-__device__ __forceinline__ float row_loss(const Distill &a, const typename T::Raw *x, const int *ids, const float *part, const float *value,
-                                          const Teacher &teacher, const Shift &t, const Shift &one, float sum, float sum1, int64_t label)
+// Sums relative to another maximum.
+template <int KIND, bool ONE_STEP>
+__device__ __forceinline__ void rebase(Sums &s, float max, float c)
 {
-    const lpmm_distill_call &c = a.c;
-    const float inv_t = 1.0f / c.temperature, log_s = logf(sum);
-    float kd = 0.0f;
-    for (int k = threadIdx.x; k < (int)c.topk; k += kWave) {
-        const float p = part[k];
-        if (p > 0.0f)
-            kd += p * (((value[k] - teacher.top) * inv_t - teacher.log_total) - (t.of_value(T::get(x[ids[k]])) * kLn2 - log_s));
-    }
-    kd = wave_sum(kd);
-    float loss = c.teacher_weight * (c.temperature * c.temperature) * kd;
-    if (a.with_label && !teacher.bad)
-        loss += c.label_weight * (logf(sum1) - one.of_value(T::get(x[label])) * kLn2);
-    return teacher.bad ? NAN : loss;
-}
-
-// The listed entries and the label, with what they take off: one thread for each id, which sums the parts of the entries with that id in
-// their order.  The rest of the row has been written, by other threads of the workgroup.
-template <typename T, int KIND>
-__device__ __forceinline__ void write_entries(const Distill &a, const typename T::Raw *x, typename T::Raw *grad, const int *ids, const float *part,
-                                              const Shift &t, const Shift &one, const Factors &f, float kt, float kl, int threads)
-{
-    const int topk = (int)a.c.topk;
-    for (int k = threadIdx.x; k <= topk; k += threads) {
-        const int id = ids[k];
-        if (id < 0)
-            continue;
-        int same = 0;
-        for (int j = 0; j <= topk; j += 4) {
-            const int4 four = *reinterpret_cast<const int4 *>(ids + j);
-            same += (four.x == id) + (four.y == id) + (four.z == id) + (four.w == id);
-        }
-        float off = k < topk ? kt * part[k] : kl;
-        if (same > 1) {
-            bool first = true;
-            for (int j = 0; j < k && first; ++j)
-                first = ids[j] != id;
-            if (!first)
-                continue;
-            for (int j = k + 1; j <= topk; ++j)
-                if (ids[j] == id)
-                    off += j < topk ? kt * part[j] : kl;
-        }
-        const float v = T::get(x[id]), e = exp2_fast(t.of_value(v));
-        const float e1 = KIND == kTwo ? exp2_fast(one.of_value(v)) : 0.0f;
-        grad[id] = T::put(smooth<KIND>(e, e1, f) - off);
-    }
-}
-
-template <typename T>
-__device__ __forceinline__ void write_zeros(typename T::Raw *grad, uint32_t vocab, int threads)
-{
-    const uint32_t whole = vocab - vocab % T::kRun;
-    for (uint32_t at = threadIdx.x * T::kRun; at < whole; at += threads * T::kRun)
-        store_run<T>(grad + at, u32x4{});
-    if (threadIdx.x < vocab - whole)
-        grad[whole + threadIdx.x] = T::put(0.0f);
+    if (s.sum == 0.0f)  // nothing yet, whatever its maximum
+        return;
+    const float f = from_to<KIND, ONE_STEP>(s.max, max, c);
+    s.sum *= f;
+    if (KIND == kSquare)
+        s.sum1 *= f * f;
+    if (KIND == kTwo)
+        s.sum1 *= from_to<KIND, ONE_STEP>(s.max, max, kLog2e);
 }
 
 // RUNS runs of 16 bytes in each thread; RUNS = 0: rows of any length, read twice.
-template <typename T, int KIND, int THREADS, int RUNS>
-__global__ __launch_bounds__(THREADS) void distill_kernel(Distill a)
+// AGAIN: the gradient call, which knows the sums.
+template <typename T, int KIND, bool AGAIN, int THREADS, int RUNS>
+__global__ __launch_bounds__(THREADS, RUNS > 4 ? 4 : 6) void distill_kernel(Distill a)
 {
     using Raw = typename T::Raw;
     constexpr uint32_t kStride = THREADS * T::kRun;
-    constexpr int kWaves = THREADS / kWave;
-    __shared__ float room[3][kWaves];
-    __shared__ Teacher teacher;
+    constexpr int kWaves = THREADS / kWave, kEntries = LPMM_DISTILL_MOST / THREADS;
+    constexpr bool kOneStep = T::kRun == 8;
+    static_assert(kWaves >= 4 && kWaves <= 16, "lanes_sum");
+    struct OfWave {
+        float max, sum, sum1, top, total, kd;
+        int fits, wrong;
+    };
+    __shared__ OfWave room[kWaves];
     extern __shared__ __attribute__((aligned(16))) int entries[];
     const lpmm_distill_call &c = a.c;
-    const bool again = a.grad_loss != nullptr;  // the gradient call: the sums are known
-    if (again && a.made && a.grad_loss[0] == 1.0f)
-        return;
-    const int places = ((int)c.topk + 1 + 3) & ~3, wave = threadIdx.x / kWave;
-    int *ids = entries;
-    float *part = reinterpret_cast<float *>(entries + places), *value = part + places;
-    const uint32_t tid = threadIdx.x, vocab = (uint32_t)c.vocab;  // below 2^31: a position and a stride past it fit 32 bits
-    const uint32_t whole = vocab - vocab % T::kRun;
     const int64_t row = blockIdx.x;
+    float scale = a.each;
+    if constexpr (AGAIN) {
+        scale *= a.grad_loss[row * a.grad_loss_stride];
+        if (a.made && scale == a.each)  // times 1
+            return;
+    }
+    if (c.reduction == LPMM_REDUCE_MEAN && c.labels)
+        scale *= c.share[0];
+    const int topk = (int)c.topk, listed = topk + 1, places = (listed + 3) & ~3;
+    int *ids = entries;
+    float *part = reinterpret_cast<float *>(entries + places);
+    const uint32_t tid = threadIdx.x, wave = tid / kWave, vocab = (uint32_t)c.vocab;  // below 2^31: a position and a stride past it fit 32 bits
     Raw *grad = c.grad ? static_cast<Raw *>(c.grad) + row * (int64_t)vocab : nullptr;
     const int64_t label = c.labels ? c.labels[row] : -1;
     const Raw *x = row_of<T>(c, row);
+    const Cut cut = Cut::of<T>(grad ? grad : x, vocab);
+    const uint32_t single = cut.single<T>(), first = cut.head + tid * T::kRun;
     auto no_part = [&] {
-        if (!again && tid == 0)
+        if (!AGAIN && tid == 0)
             c.row_loss[row] = 0.0f;
-        if (grad)
-            write_zeros<T>(grad, vocab, THREADS);
+        if (!grad)
+            return;
+        for (uint32_t at = first; at < cut.end; at += kStride)
+            store_run_once<T>(grad + at, u32x4{});
+        if (single < vocab)
+            grad[single] = T::put(0.0f);
     };
     if (c.labels && label == c.ignore_index)
         return no_part();
 
-    u32x4 held[RUNS > 0 ? RUNS : 1];
-    float last = -INFINITY;  // of the values past the last whole run, one to a thread
-    if (tid < vocab - whole)
-        last = T::get(x[whole + tid]);
-    if constexpr (RUNS > 0) {
+    // everything that the row needs is asked for before anything is looked at
+    Entry entry[kEntries];
 #pragma unroll
-        for (int i = 0; i < RUNS; ++i) {
-            const uint32_t at = i * kStride + tid * T::kRun;
-            held[i] = u32x4{T::kNoValue, T::kNoValue, T::kNoValue, T::kNoValue};
-            if (at < whole)
-                held[i] = load_run<T>(x + at);
+    for (int i = 0; i < kEntries; ++i) {
+        entry[i].id = -1;
+        if (i * THREADS + (int)tid < topk)
+            entry[i].load(c, row * topk + i * THREADS + tid);
+    }
+    const bool label_wrong = c.labels && (label < 0 || label >= c.vocab), has_label = a.with_label && !label_wrong;
+    const uint32_t label_bits = load_bits<T>(x + (has_label ? label : 0)), alone_bits = load_bits<T>(x + (single < vocab ? single : 0));
+    u32x4 held[RUNS > 0 ? RUNS : 1];
+    if constexpr (RUNS > 0) {
+        auto hold = [&](auto &&load) {
+#pragma unroll
+            for (int i = 0; i < RUNS; ++i) {  // past the row's end its last run, so that no load is a branch
+                const uint32_t at = min(first + i * kStride, cut.end - T::kRun);
+                held[i] = load(reinterpret_cast<const Raw *>(reinterpret_cast<const char *>(x) + at * (uint32_t)sizeof(Raw)));
+            }
+        };
+        if (cut.end > cut.head) {
+            // the assembler comments keep the compiler from making one set of loads of the two, without the hint
+            if (a.far) {
+                asm volatile("; once");
+                hold([](const Raw *p) { return load_run_once<T>(p); });
+                asm volatile("; once");
+            } else {
+                asm volatile("; again");
+                hold([](const Raw *p) { return load_run<T>(p); });
+                asm volatile("; again");
+            }
         }
     }
-    // each held run that a thread of the workgroup has
+    bool wrong = label_wrong;
+    const bool has_entries = (int)(wave * kWave) < topk;
+    if (has_entries) {
+#pragma unroll
+        for (int i = 0; i < kEntries; ++i)
+            if (i * THREADS < topk) {
+                wrong |= entry[i].id >= c.vocab;
+                if (entry[i].id >= c.vocab)
+                    entry[i].id = -1;
+                entry[i].x = load_bits<T>(x + (entry[i].id >= 0 ? entry[i].id : 0));
+            }
+    }
+    // each run of the thread, from where it is held; or read again, for what is seldom done (and for rows that are not held)
+    auto read_runs = [&](auto &&body) {
+#pragma unroll 1
+        for (uint32_t at = first; at < cut.end; at += kStride)
+            body(at, load_run<T>(x + at));
+    };
     auto runs = [&](auto &&body) {
         if constexpr (RUNS > 0) {
 #pragma unroll
             for (int i = 0; i < RUNS; ++i)
-                if (i * kStride < whole)
-                    body(i, i * kStride + tid * T::kRun, held[i]);
+                if (cut.head + i * kStride < cut.end) {
+                    const uint32_t at = first + i * kStride;
+                    asm volatile("" : "+v"(held[i]));  // unpacked anew each time: the floats of a row do not fit
+                    body(at, at < cut.end ? held[i] : u32x4{T::kNoValue, T::kNoValue, T::kNoValue, T::kNoValue});
+                }
         } else {
-            for (uint32_t at = tid * T::kRun; at < whole; at += kStride)
-                body(0, at, load_run<T>(x + at));
+            read_runs(body);
         }
     };
-    if (wave == 0)
-        read_teacher(a, row, label, ids, part, value, &teacher);
-
-    float max, sum, sum1;
-    if (again) {
+    const float alone = single < vocab ? from_bits<T>(alone_bits) : -INFINITY;
+    const float ct = KIND == kOne && c.temperature == 1.0f ? kLog2e : kLog2e / c.temperature;
+    const float inv_t = 1.0f / c.temperature;
+    float top = -INFINITY, total = 0.0f;
+    auto look = [&] {  // the wave's part of the teacher's softmax
+        if (!has_entries)
+            return;
+#pragma unroll
+        for (int i = 0; i < kEntries; ++i)
+            if (i * THREADS < topk) {
+                const int k = i * THREADS + tid;
+                entry[i].t = -INFINITY;
+                if (k < topk) {
+                    if (entry[i].id >= 0)
+                        entry[i].t = entry[i].value_of(c, row * topk + k);
+                    wrong |= !(entry[i].t < INFINITY);
+                    ids[k] = (int)entry[i].id;
+                }
+                top = fmaxf(top, entry[i].t);
+            }
+        top = wave_max(top);
+#pragma unroll
+        for (int i = 0; i < kEntries; ++i)
+            if (i * THREADS < topk)
+                total += top > -INFINITY ? expf((entry[i].t - top) * inv_t) : 0.0f;
+        total = wave_sum(total);
+    };
+    if ((int)tid < places - topk)
+        ids[topk + tid] = tid == 0 && has_label ? (int)label : -1;
+    Sums all;
+    if constexpr (AGAIN) {
+        look();
         const float4 kept = reinterpret_cast<const float4 *>(c.row_stats)[row];
-        max = kept.x, sum = kept.y, sum1 = kept.z;
+        all = {kept.x, kept.y, kept.z};
+        const bool any_wrong = __any(wrong);
+        if (tid % kWave == 0)
+            room[wave] = {0.0f, 0.0f, 0.0f, top, total, 0.0f, 0, any_wrong};
         __syncthreads();
     } else {
-        float m = last;
-        runs([&](int, uint32_t, u32x4 r) { m = run_max<T>(r, m); });
-        m = wave_max(m);
-        if (tid % kWave == 0)
-            room[0][wave] = m;
-        __syncthreads();
-        max = room[0][0];
-#pragma unroll
-        for (int w = 1; w < kWaves; ++w)
-            max = fmaxf(max, room[0][w]);
-    }
-    if (!teacher.some && !a.with_label && !teacher.bad)  // neither term has anything to say of the row
-        return no_part();
-    if (max == -INFINITY)
-        max = NAN;  // no softmax: everything becomes NaN, as 0 / 0 does
-    Shift one = Shift::of<T>(max, kLog2e), t = KIND == kOne && c.temperature == 1.0f ? one : Shift::of<T>(max, kLog2e / c.temperature);
-    const bool one_step = t.one_step() && one.one_step();
-    if (!one_step)
-        t.m = one.m = NAN;
-    if (!again) {
-        float s = exp2_fast(t.of_value(last)), s1 = KIND == kSquare ? s * s : KIND == kTwo ? exp2_fast(one.of_value(last)) : 0.0f;
-        if (one_step)
-            runs([&](int, uint32_t, u32x4 r) { run_sums<T, KIND, true>(r, t, one, s, s1); });
-        else
-            runs([&](int, uint32_t, u32x4 r) { run_sums<T, KIND, false>(r, t, one, s, s1); });
-        s = wave_sum(s);
+        // Each thread's exponentials are relative to the largest of its first run and its single value, so that sums grow as
+        // the runs arrive, with no pass for the row's largest value before.  That fits unless a later value is so much larger that a
+        // sum leaves its range, or the first run says nothing.
+        float m = alone;
+        if (first < cut.end)
+            m = run_max<T>(RUNS > 0 ? held[0] : load_run<T>(x + first), m);
+        const bool none = m == -INFINITY;
+        Sums s = {none ? 0.0f : m, 0.0f, 0.0f};
+        Shift t, one;
+        shifts<T, KIND>(s.max, ct, t, one);
+        s.sum = exp2_fast(kOneStep ? fmaf(alone, t.c, -t.m) : (alone - t.max) * t.c);
+        s.sum1 = KIND == kSquare ? s.sum * s.sum : KIND == kTwo ? exp2_fast(kOneStep ? fmaf(alone, one.c, -one.m) : (alone - one.max) * one.c) : 0.0f;
+        runs([&](uint32_t, u32x4 r) { run_sums<T, KIND, kOneStep>(r, t, one, s.sum, s.sum1); });
+        // s.sum is NaN where t.m is: values too large for one step
+        const bool fit = !(none && first < cut.end) && s.sum < 0x1p30f && (KIND != kTwo || s.sum1 < 0x1p30f);
+        const float most = wave_max(s.sum == 0.0f ? -INFINITY : s.max);
+        rebase<KIND, kOneStep>(s, most, ct);
+        s.sum = wave_sum(s.sum);
         if (KIND != kOne)
-            s1 = wave_sum(s1);
+            s.sum1 = wave_sum(s.sum1);
+        look();
+        const bool all_fit = __all(fit), any_wrong = __any(wrong);
         if (tid % kWave == 0)
-            room[1][wave] = s, room[2][wave] = s1;
+            room[wave] = {most, s.sum, s.sum1, top, total, 0.0f, all_fit, any_wrong};
         __syncthreads();
-        sum = room[1][0], sum1 = room[2][0];
-#pragma unroll
-        for (int w = 1; w < kWaves; ++w)
-            sum += room[1][w], sum1 += room[2][w];
+        const OfWave of = room[tid % kWaves];
+        const bool fine = __all(of.fits);
+        all.max = lanes_max<kWaves>(of.max);
+        s = {of.max, of.sum, of.sum1};
+        rebase<KIND, kOneStep>(s, all.max, ct);
+        all.sum = lanes_sum<kWaves>(s.sum);
+        all.sum1 = lanes_sum<kWaves>(s.sum1);
+        if (!fine || !(all.sum < 0x1p30f)) {  // the largest value first, then differences to it
+            __syncthreads();
+            float largest = alone;
+            read_runs([&](uint32_t, u32x4 r) { largest = run_max<T>(r, largest); });
+            largest = wave_max(largest);
+            if (tid % kWave == 0)
+                room[wave].max = largest;
+            __syncthreads();
+            largest = lanes_max<kWaves>(room[tid % kWaves].max);
+            if (largest == -INFINITY)
+                largest = NAN;  // no softmax: everything becomes NaN, as 0 / 0 does
+            shifts<T, KIND>(largest, ct, t, one);
+            s.sum = exp2_fast(t.of_value(alone));
+            s.sum1 = KIND == kSquare ? s.sum * s.sum : KIND == kTwo ? exp2_fast(one.of_value(alone)) : 0.0f;
+            if (kOneStep && t.one_step())
+                read_runs([&](uint32_t, u32x4 r) { run_sums<T, KIND, kOneStep>(r, t, one, s.sum, s.sum1); });
+            else
+                read_runs([&](uint32_t, u32x4 r) { run_sums<T, KIND, false>(r, t, one, s.sum, s.sum1); });
+            s.sum = wave_sum(s.sum);
+            if (KIND != kOne)
+                s.sum1 = wave_sum(s.sum1);
+            if (tid % kWave == 0)
+                room[wave].sum = s.sum, room[wave].sum1 = s.sum1;
+            __syncthreads();
+            all = {largest, lanes_sum<kWaves>(room[tid % kWaves].sum), lanes_sum<kWaves>(room[tid % kWaves].sum1)};
+        }
         if (KIND == kOne)
-            sum1 = sum;
-        if (wave == 0) {
-            const float loss = row_loss<T>(a, x, ids, part, value, teacher, t, one, sum, sum1, label);
-            if (tid == 0) {
-                c.row_loss[row] = loss;
-                if (c.row_stats)
-                    reinterpret_cast<float4 *>(c.row_stats)[row] = make_float4(max, sum, sum1, 0.0f);
+            all.sum1 = all.sum;
+    }
+    // the teacher's softmax from the waves' parts of it
+    const OfWave of = room[tid % kWaves];
+    const bool bad = __any(of.wrong);
+    top = lanes_max<kWaves>(of.top);
+    const bool some = top > -INFINITY;
+    total = lanes_sum<kWaves>(of.total > 0.0f ? of.total * expf((of.top - top) * inv_t) : 0.0f);
+    if (!some && !a.with_label && !bad)  // neither term has anything to say of the row
+        return no_part();
+    Shift t, one;
+    shifts<T, KIND>(all.max, ct, t, one);
+    const float kt = bad ? NAN : some ? scale * c.teacher_weight * c.temperature : 0.0f;
+    const float kl = a.with_label ? scale * c.label_weight : 0.0f;
+    if ((int)(wave * kWave) < topk) {
+        const float inv_total = some ? 1.0f / total : 0.0f, log_total = some ? logf(total) : 0.0f, log_s = logf(all.sum);
+        float kd = 0.0f;
+#pragma unroll
+        for (int i = 0; i < kEntries; ++i) {
+            const int k = i * THREADS + tid;
+            if (k < topk) {
+                const float z = (entry[i].t - top) * inv_t, p = some ? expf(z) * inv_total : 0.0f;
+                if (p > 0.0f)
+                    kd += p * ((z - log_total) - (t.of_value(from_bits<T>(entry[i].x)) * kLn2 - log_s));
+                part[k] = kt * p;
             }
         }
+        if (!AGAIN) {
+            kd = wave_sum(kd);
+            if (tid % kWave == 0)
+                room[wave].kd = kd;
+        }
+    }
+    if (tid == 0) {
+        part[topk] = kl;
+        if (!AGAIN && c.row_stats)
+            reinterpret_cast<float4 *>(c.row_stats)[row] = make_float4(all.max, all.sum, all.sum1, 0.0f);
+    }
+    const Factors f = {(KIND == kOne ? kt + kl : kt) / all.sum, KIND == kOne ? 0.0f : kl / all.sum1};
+    auto value_of = [&](float v) {
+        return smooth<KIND>(exp2_fast(t.of_value(v)), KIND == kTwo ? exp2_fast(one.of_value(v)) : 0.0f, f);
+    };
+    if (grad) {
+        if (!kOneStep || t.one_step())
+            runs([&](uint32_t at, u32x4 r) {
+                const u32x4 g = run_grad<T, KIND, kOneStep>(r, t, one, f);
+                if (at < cut.end)
+                    store_run_once<T>(grad + at, g);
+            });
+        else
+            read_runs([&](uint32_t at, u32x4 r) { store_run_once<T>(grad + at, run_grad<T, KIND, false>(r, t, one, f)); });
+        if (single < vocab)
+            grad[single] = T::put(value_of(alone));
+    }
+    __syncthreads();  // entries in shared memory; what the workgroup wrote of the row comes before what follows
+    if (!AGAIN && tid == 0) {
+        float loss = 0.0f;
+        for (int w = 0; w < kWaves && w * kWave < topk; ++w)
+            loss += room[w].kd;
+        loss *= c.teacher_weight * (c.temperature * c.temperature);
+        if (a.with_label)
+            loss += c.label_weight * (logf(all.sum1) - one.of_value(from_bits<T>(label_bits)) * kLn2);
+        c.row_loss[row] = bad ? NAN : loss;
     }
     if (!grad)
         return;
-    const float each = c.reduction == LPMM_REDUCE_MEAN && c.labels ? c.share[0] : a.each;
-    const float scale = each * (again ? a.grad_loss[row * a.grad_loss_stride] : 1.0f);
-    const float kt = teacher.bad ? NAN : teacher.some ? scale * c.teacher_weight * c.temperature : 0.0f;
-    const float kl = a.with_label ? scale * c.label_weight : 0.0f;
-    const Factors f = {(KIND == kOne ? kt + kl : kt) / sum, KIND == kOne ? 0.0f : kl / sum1};
-    auto write = [&](auto steps) {
-        runs([&](int, uint32_t at, u32x4 r) {
-            const u32x4 g = run_grad<T, KIND, decltype(steps)::value>(r, t, one, f);
-            if (at < whole)
-                store_run<T>(grad + at, g);
-        });
-    };
-    if (one_step)
-        write(std::true_type());
-    else
-        write(std::false_type());
-    if (tid < vocab - whole) {
-        const float e = exp2_fast(t.of_value(last)), e1 = KIND == kTwo ? exp2_fast(one.of_value(last)) : 0.0f;
-        grad[whole + tid] = T::put(smooth<KIND>(e, e1, f));
+    // the listed entries and the label again, with what they take off: one thread for each id
+    float off;
+#pragma unroll
+    for (int i = 0; i < kEntries; ++i) {
+        const int k = i * THREADS + tid;
+        if (k < topk && entry[i].id >= 0 && takes_off(ids, part, listed, k, off))
+            grad[entry[i].id] = T::put(value_of(from_bits<T>(entry[i].x)) - off);
     }
-    // The entries' places are written again: the wait lets the stores above be done first.
-    __builtin_amdgcn_s_waitcnt(0);
-    __syncthreads();
-    write_entries<T, KIND>(a, x, grad, ids, part, t, one, f, kt, kl, THREADS);
+    if (tid == 0 && ids[topk] >= 0 && takes_off(ids, part, listed, topk, off))
+        grad[label] = T::put(value_of(from_bits<T>(label_bits)) - off);
 }
 
 constexpr int kSumThreads = 1024;
@@ -390,8 +547,10 @@ __global__ __launch_bounds__(kSumThreads) void distill_share_kernel(const int64_
 {
     __shared__ double room[kSumThreads / kWave];
     int64_t n = 0;
-    for (int64_t i = threadIdx.x; i < rows; i += kSumThreads)
-        n += labels[i] != ignore;
+    for (int64_t i = threadIdx.x; i < rows; i += 8 * kSumThreads)
+#pragma unroll
+        for (int j = 0; j < 8; ++j)  // loads that do not wait for each other
+            n += i + j * kSumThreads < rows && labels[i + j * kSumThreads] != ignore;
     const double all = block_sum_f64<kSumThreads>((double)n, room);
     if (threadIdx.x == 0)
         share[0] = all > 0.0 ? (float)(1.0 / all) : 0.0f;
@@ -402,8 +561,10 @@ __global__ __launch_bounds__(kSumThreads) void distill_sum_kernel(const float *r
 {
     __shared__ double room[kSumThreads / kWave];
     double s = 0.0;
-    for (int64_t i = threadIdx.x; i < rows; i += kSumThreads)
-        s += (double)row_loss[i];
+    for (int64_t i = threadIdx.x; i < rows; i += 8 * kSumThreads)
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            s += i + j * kSumThreads < rows ? (double)row_loss[i + j * kSumThreads] : 0.0;
     s = block_sum_f64<kSumThreads>(s, room);
     if (threadIdx.x == 0)
         loss[0] = (float)(s * (share ? (double)share[0] : each));
@@ -450,7 +611,8 @@ Distill arguments(const lpmm_distill_call &c)
     if (c.teacher_weight == 0.0f)
         a.c.topk = 0;  // a term without weight is not looked at
     a.with_label = c.labels && c.label_weight != 0.0f;
-    a.each = c.reduction == LPMM_REDUCE_MEAN && c.rows > 0 ? (float)(1.0 / (double)c.rows) : 1.0f;
+    a.far = c.rows * c.vocab * (c.type == LPMM_TYPE_F32 ? 4 : 2) > kLastLevel;
+    a.each = c.reduction == LPMM_REDUCE_MEAN && !c.labels ? (float)(1.0 / (double)c.rows) : 1.0f;
     return a;
 }
 
@@ -458,7 +620,10 @@ template <typename T, int KIND, int THREADS, int RUNS>
 void launch(const Distill &a, hipStream_t stream)
 {
     const int places = ((int)a.c.topk + 1 + 3) & ~3;
-    distill_kernel<T, KIND, THREADS, RUNS><<<(unsigned)a.c.rows, THREADS, places * 12, stream>>>(a);
+    if (a.grad_loss)
+        distill_kernel<T, KIND, true, THREADS, RUNS><<<(unsigned)a.c.rows, THREADS, places * 8, stream>>>(a);
+    else
+        distill_kernel<T, KIND, false, THREADS, RUNS><<<(unsigned)a.c.rows, THREADS, places * 8, stream>>>(a);
 }
 
 template <typename T, int KIND>

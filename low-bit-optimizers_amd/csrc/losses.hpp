@@ -89,18 +89,25 @@ struct BF16 {
 
 // 16 bytes of values at an address that only their type aligns: rows of odd lengths start anywhere, and the hardware takes a 16-byte access
 // at any address of device memory.
+typedef uint32_t u32x4_any __attribute__((ext_vector_type(4), aligned(2)));
+
 template <typename T>
 __device__ __forceinline__ u32x4 load_run(const typename T::Raw *p)
 {
-    u32x4 r;
-    __builtin_memcpy(&r, p, sizeof r);
-    return r;
+    return *reinterpret_cast<const u32x4_any *>(p);
+}
+
+// What is read once, of an array that no cache holds.
+template <typename T>
+__device__ __forceinline__ u32x4 load_run_once(const typename T::Raw *p)
+{
+    return __builtin_nontemporal_load(reinterpret_cast<const u32x4_any *>(p));
 }
 
 template <typename T>
-__device__ __forceinline__ void store_run(typename T::Raw *p, u32x4 r)
+__device__ __forceinline__ void store_run_once(typename T::Raw *p, u32x4 r)
 {
-    __builtin_memcpy(p, &r, sizeof r);
+    __builtin_nontemporal_store(r, reinterpret_cast<u32x4_any *>(p));
 }
 
 // 2^x, off by one unit in the last place at most; results below the smallest normal number are 0
@@ -114,6 +121,31 @@ __device__ __forceinline__ float wave_sum(float v)
     v += dpp_f32<0x140>(v);  // row_mirror
     v += __shfl_xor(v, 16, kWave);
     v += __shfl_xor(v, 32, kWave);
+    return v;
+}
+
+// Sum and maximum over N neighbouring lanes (4, 8 or 16), in all of them: what N waves left, read by lane i from place i % N.
+template <int N>
+__device__ __forceinline__ float lanes_sum(float v)
+{
+    v += dpp_f32<0xB1>(v);
+    v += dpp_f32<0x4E>(v);
+    if constexpr (N >= 8)
+        v += dpp_f32<0x141>(v);
+    if constexpr (N >= 16)
+        v += dpp_f32<0x140>(v);
+    return v;
+}
+
+template <int N>
+__device__ __forceinline__ float lanes_max(float v)
+{
+    v = fmaxf(v, dpp_f32<0xB1>(v));
+    v = fmaxf(v, dpp_f32<0x4E>(v));
+    if constexpr (N >= 8)
+        v = fmaxf(v, dpp_f32<0x141>(v));
+    if constexpr (N >= 16)
+        v = fmaxf(v, dpp_f32<0x140>(v));
     return v;
 }
 
