@@ -255,12 +255,12 @@ __device__ __forceinline__ void rebase(Sums &s, float max, float c)
 
 // RUNS runs of 16 bytes in each thread; RUNS = 0: rows of any length, read twice.
 // AGAIN: the gradient call, which knows the sums.
-template <typename T, int KIND, bool AGAIN, int THREADS, int RUNS>
-__global__ __launch_bounds__(THREADS, RUNS > 4 ? 4 : 6) void distill_kernel(Distill a)
+template <typename T, int KIND, bool AGAIN, int THREADS, int RUNS, int WAVES>
+__global__ __launch_bounds__(THREADS, WAVES) void distill_kernel(Distill a)
 {
     using Raw = typename T::Raw;
     constexpr uint32_t kStride = THREADS * T::kRun;
-    constexpr int kWaves = THREADS / kWave, kEntries = LPMM_DISTILL_MOST / THREADS;
+    constexpr int kWaves = THREADS / kWave;
     constexpr bool kOneStep = T::kRun == 8;
     static_assert(kWaves >= 4 && kWaves <= 16, "lanes_sum");
     struct OfWave {
@@ -302,13 +302,11 @@ __global__ __launch_bounds__(THREADS, RUNS > 4 ? 4 : 6) void distill_kernel(Dist
         return no_part();
 
     // everything that the row needs is asked for before anything is looked at
-    Entry entry[kEntries];
-#pragma unroll
-    for (int i = 0; i < kEntries; ++i) {
-        entry[i].id = -1;
-        if (i * THREADS + (int)tid < topk)
-            entry[i].load(c, row * topk + i * THREADS + tid);
-    }
+    Entry entry;  // one to a thread: topk is at most THREADS
+    const bool has_entry = (int)tid < topk;
+    entry.id = -1;
+    if (has_entry)
+        entry.load(c, row * topk + tid);
     const bool label_wrong = c.labels && (label < 0 || label >= c.vocab), has_label = a.with_label && !label_wrong;
     const uint32_t label_bits = load_bits<T>(x + (has_label ? label : 0)), alone_bits = load_bits<T>(x + (single < vocab ? single : 0));
     u32x4 held[RUNS > 0 ? RUNS : 1];
@@ -336,14 +334,10 @@ __global__ __launch_bounds__(THREADS, RUNS > 4 ? 4 : 6) void distill_kernel(Dist
     bool wrong = label_wrong;
     const bool has_entries = (int)(wave * kWave) < topk;
     if (has_entries) {
-#pragma unroll
-        for (int i = 0; i < kEntries; ++i)
-            if (i * THREADS < topk) {
-                wrong |= entry[i].id >= c.vocab;
-                if (entry[i].id >= c.vocab)
-                    entry[i].id = -1;
-                entry[i].x = load_bits<T>(x + (entry[i].id >= 0 ? entry[i].id : 0));
-            }
+        wrong |= entry.id >= c.vocab;
+        if (entry.id >= c.vocab)
+            entry.id = -1;
+        entry.x = load_bits<T>(x + (entry.id >= 0 ? entry.id : 0));
     }
     // each run of the thread, from where it is held; or read again, for what is seldom done (and for rows that are not held)
     auto read_runs = [&](auto &&body) {
@@ -371,25 +365,12 @@ __global__ __launch_bounds__(THREADS, RUNS > 4 ? 4 : 6) void distill_kernel(Dist
     auto look = [&] {  // the wave's part of the teacher's softmax
         if (!has_entries)
             return;
-#pragma unroll
-        for (int i = 0; i < kEntries; ++i)
-            if (i * THREADS < topk) {
-                const int k = i * THREADS + tid;
-                entry[i].t = -INFINITY;
-                if (k < topk) {
-                    if (entry[i].id >= 0)
-                        entry[i].t = entry[i].value_of(c, row * topk + k);
-                    wrong |= !(entry[i].t < INFINITY);
-                    ids[k] = (int)entry[i].id;
-                }
-                top = fmaxf(top, entry[i].t);
-            }
-        top = wave_max(top);
-#pragma unroll
-        for (int i = 0; i < kEntries; ++i)
-            if (i * THREADS < topk)
-                total += top > -INFINITY ? expf((entry[i].t - top) * inv_t) : 0.0f;
-        total = wave_sum(total);
+        entry.t = entry.id >= 0 ? entry.value_of(c, row * topk + tid) : -INFINITY;
+        wrong |= !(entry.t < INFINITY);
+        if (has_entry)
+            ids[tid] = (int)entry.id;
+        top = wave_max(entry.t);
+        total = wave_sum(top > -INFINITY ? expf((entry.t - top) * inv_t) : 0.0f);
     };
     if ((int)tid < places - topk)
         ids[topk + tid] = tid == 0 && has_label ? (int)label : -1;
@@ -478,19 +459,11 @@ __global__ __launch_bounds__(THREADS, RUNS > 4 ? 4 : 6) void distill_kernel(Dist
     const float kl = a.with_label ? scale * c.label_weight : 0.0f;
     if ((int)(wave * kWave) < topk) {
         const float inv_total = some ? 1.0f / total : 0.0f, log_total = some ? logf(total) : 0.0f, log_s = logf(all.sum);
-        float kd = 0.0f;
-#pragma unroll
-        for (int i = 0; i < kEntries; ++i) {
-            const int k = i * THREADS + tid;
-            if (k < topk) {
-                const float z = (entry[i].t - top) * inv_t, p = some ? expf(z) * inv_total : 0.0f;
-                if (p > 0.0f)
-                    kd += p * ((z - log_total) - (t.of_value(from_bits<T>(entry[i].x)) * kLn2 - log_s));
-                part[k] = kt * p;
-            }
-        }
+        const float z = (entry.t - top) * inv_t, p = some ? expf(z) * inv_total : 0.0f;
+        if (has_entry)
+            part[tid] = kt * p;
         if (!AGAIN) {
-            kd = wave_sum(kd);
+            const float kd = wave_sum(p > 0.0f ? p * ((z - log_total) - (t.of_value(from_bits<T>(entry.x)) * kLn2 - log_s)) : 0.0f);
             if (tid % kWave == 0)
                 room[wave].kd = kd;
         }
@@ -530,12 +503,8 @@ __global__ __launch_bounds__(THREADS, RUNS > 4 ? 4 : 6) void distill_kernel(Dist
         return;
     // the listed entries and the label again, with what they take off: one thread for each id
     float off;
-#pragma unroll
-    for (int i = 0; i < kEntries; ++i) {
-        const int k = i * THREADS + tid;
-        if (k < topk && entry[i].id >= 0 && takes_off(ids, part, listed, k, off))
-            grad[entry[i].id] = T::put(value_of(from_bits<T>(entry[i].x)) - off);
-    }
+    if (has_entry && entry.id >= 0 && takes_off(ids, part, listed, tid, off))
+        grad[entry.id] = T::put(value_of(from_bits<T>(entry.x)) - off);
     if (tid == 0 && ids[topk] >= 0 && takes_off(ids, part, listed, topk, off))
         grad[label] = T::put(value_of(from_bits<T>(label_bits)) - off);
 }
@@ -616,34 +585,43 @@ Distill arguments(const lpmm_distill_call &c)
     return a;
 }
 
-template <typename T, int KIND, int THREADS, int RUNS>
+template <typename T, int KIND, int THREADS, int RUNS, int WAVES>
 void launch(const Distill &a, hipStream_t stream)
 {
     const int places = ((int)a.c.topk + 1 + 3) & ~3;
     if (a.grad_loss)
-        distill_kernel<T, KIND, true, THREADS, RUNS><<<(unsigned)a.c.rows, THREADS, places * 8, stream>>>(a);
+        distill_kernel<T, KIND, true, THREADS, RUNS, WAVES><<<(unsigned)a.c.rows, THREADS, places * 8, stream>>>(a);
     else
-        distill_kernel<T, KIND, false, THREADS, RUNS><<<(unsigned)a.c.rows, THREADS, places * 8, stream>>>(a);
+        distill_kernel<T, KIND, false, THREADS, RUNS, WAVES><<<(unsigned)a.c.rows, THREADS, places * 8, stream>>>(a);
 }
 
 template <typename T, int KIND>
 void launch_kind(const Distill &a, hipStream_t stream)
 {
     const int64_t runs = a.c.vocab / T::kRun;  // whole ones
+    const auto fits = [&](int threads, int each) { return runs <= threads * each && a.c.topk <= threads; };
+    // Small workgroups that fill a compute unit several times over, down to two with 64 registers a thread, then one with twice as many.  bf16 rows,
+    // loss and gradient of 1 GB (16 KB rows: 268 MB), us with the neighbouring choices: 8192 values 60 (256 x 8 59, 512 x 8 76), 16384: 107 (512 x 8
+    // 111), 32000: 196 (256 x 16 200, 1024 x 7 204), 50257: 204 (1024 x 8 210, 512 x 16 215), 65536: 196 (512 x 16 194, 1024 x 16 234).
+    // Fewer rows than compute units: the most threads a row can have.
     if (a.c.rows < 256) {
-        if (runs <= 1024 * 4)
-            return launch<T, KIND, 1024, 4>(a, stream);
+        if (fits(1024, 4))
+            return launch<T, KIND, 1024, 4, 4>(a, stream);
     } else {
-        if (runs <= 256 * 4)
-            return launch<T, KIND, 256, 4>(a, stream);
-        if (runs <= 256 * 16)
-            return launch<T, KIND, 256, 16>(a, stream);
-        if (runs <= 512 * 16)
-            return launch<T, KIND, 512, 16>(a, stream);
+        if (fits(256, 4))
+            return launch<T, KIND, 256, 4, 8>(a, stream);
+        if (fits(256, 8))
+            return launch<T, KIND, 256, 8, 6>(a, stream);
+        if (fits(512, 8))
+            return launch<T, KIND, 512, 8, 6>(a, stream);
     }
-    if (runs <= 1024 * 16)
-        return launch<T, KIND, 1024, 16>(a, stream);
-    launch<T, KIND, 1024, 0>(a, stream);
+    if (fits(1024, 7))
+        return launch<T, KIND, 1024, 7, 8>(a, stream);
+    if (fits(1024, 8))
+        return launch<T, KIND, 1024, 8, 8>(a, stream);
+    if (fits(1024, 16))
+        return launch<T, KIND, 1024, 16, 4>(a, stream);
+    launch<T, KIND, 1024, 0, 4>(a, stream);
 }
 
 template <typename T>
