@@ -6,155 +6,296 @@
 // The gradient needs the counts of the whole group, so the logits are read twice: by the call that sums the probabilities and counts the
 // picks, and by the one that writes the gradient, which makes the probabilities again rather than read them back (4 bytes a value).
 //
-// A token's logits lie across 2^l lanes of a wave, 4 or 16 side by side in each, and its maximum and sums are exchanges between those lanes.  A
-// thread keeps the sums of its experts' probabilities over all the tokens that pass through it; waves and workgroups are joined in a
-// fixed order.  Counts are integers: the order of their atomics, in shared memory only, does not change them.
+// A token's logits lie across up to 16 neighbouring lanes, in chunks of 16 bytes a lane, so that its maximum and its sums are exchanges
+// within a row of lanes (no shared memory) and every load of a wave covers whole stretches of several tokens.  A thread keeps the sums of
+// its experts' probabilities over all the tokens that pass through it; lanes, waves and workgroups are joined in a fixed order.  Counts are
+// integers: the order of their atomics, in shared memory only, does not change them.
 #include "losses.hpp"
 
 namespace lpmm {
 namespace {
 
-constexpr int kBalThreads = 256;
-constexpr int kBalWaves = kBalThreads / kWave;
-constexpr int64_t kBalParts = 256;  // workgroups a group's tokens are divided among at most
+constexpr int kBalThreads = 256, kBalWaves = kBalThreads / kWave, kLanes = 16;
+constexpr int kJoinThreads = 1024, kJoinColumns = 16, kJoinSlices = kJoinThreads / kJoinColumns;
 
 struct Balance {
     lpmm_balance_call c;
     const float *grad_loss;
     int64_t parts, per;  // workgroups to a group, tokens to a workgroup
     int lanes;           // lanes to a token
-    // parts of the sums, [groups][parts]: of probabilities and picks [experts], of lse^2, of tokens that count (-1 - n for n with a wrong id among theirs); the groups' losses
+    int tiles;           // workgroups that join a group
+    // parts of the sums, [groups][parts]: of probabilities and picks [experts], of lse^2, of tokens that count (-1 - n for n with a wrong
+    // id among theirs); parts of the loss [groups][tiles]; how many of these are there
     float *prob;
     int32_t *picked;
     double *square;
     int32_t *seen;
-    double *group_loss;
+    double *loss_part;
+    uint32_t *done;
 };
 
 struct Split {
-    int64_t parts, per;
+    int64_t parts, per, tiles;
 };
 
-// Tokens to a workgroup: 64 at least, so that what it joins at its end is little beside what it reads.
-Split split(int64_t groups, int64_t tokens)
+// Tokens to a workgroup of the sums: 128 at least, so that what it joins at its end is little beside what it reads; 1024 workgroups at most,
+// four for each compute unit.  One workgroup alone joins its own sums, without a second launch.
+Split split(int64_t groups, int64_t tokens, int64_t experts)
 {
-    int64_t parts = (tokens + 63) / 64;
-    const int64_t most = groups >= kBalParts ? 1 : kBalParts / groups;
-    if (parts > most)
-        parts = most;
-    if (parts < 1)
-        parts = 1;
-    return {parts, (tokens + parts - 1) / parts};
+    const int64_t most = groups >= 1024 ? 1 : 1024 / groups;
+    int64_t parts = (tokens + 127) / 128;
+    parts = parts > most ? most : parts < 1 ? 1 : parts;
+    return {parts, (tokens + parts - 1) / parts, (experts + kJoinColumns - 1) / kJoinColumns};
 }
 
-__device__ __forceinline__ float spread_max(float v, int lanes)
+// Over the lanes of a token, 2^l of them at most 16, in all of them.
+__device__ __forceinline__ float token_max(float v, int lanes)
 {
-    for (int o = lanes >> 1; o > 0; o >>= 1)
-        v = fmaxf(v, __shfl_xor(v, o, kWave));
+    if (lanes > 1)
+        v = fmaxf(v, dpp_f32<0xB1>(v));
+    if (lanes > 2)
+        v = fmaxf(v, dpp_f32<0x4E>(v));
+    if (lanes > 4)
+        v = fmaxf(v, dpp_f32<0x141>(v));
+    if (lanes > 8)
+        v = fmaxf(v, dpp_f32<0x140>(v));
     return v;
 }
 
-__device__ __forceinline__ float spread_sum(float v, int lanes)
+__device__ __forceinline__ float token_sum(float v, int lanes)
 {
-    for (int o = lanes >> 1; o > 0; o >>= 1)
-        v += __shfl_xor(v, o, kWave);
+    if (lanes > 1)
+        v += dpp_f32<0xB1>(v);
+    if (lanes > 2)
+        v += dpp_f32<0x4E>(v);
+    if (lanes > 4)
+        v += dpp_f32<0x141>(v);
+    if (lanes > 8)
+        v += dpp_f32<0x140>(v);
     return v;
 }
 
-// The run of logits that a lane holds of a token; past the last expert -infinity, whose probability is 0.
-template <typename T, int RUN>
-__device__ __forceinline__ void load_logits(const typename T::Raw *x, int held, float (&v)[RUN])
+// Chunk i of a lane: experts [first + i * step, ...), RUN of them where the token has so many.
+struct Place {
+    int first, step, experts;
+    template <typename T>
+    static __device__ __forceinline__ Place of(const Balance &a)
+    {
+        return {(int)(threadIdx.x & (a.lanes - 1)) * T::kRun, a.lanes * T::kRun, (int)a.c.experts};
+    }
+    __device__ __forceinline__ int held(int chunk) const { return experts - first - chunk * step; }
+};
+
+// A lane's chunks of a token's logits; past the last expert -infinity, whose probability is 0.
+template <typename T, int CHUNKS>
+__device__ __forceinline__ void load_logits(const typename T::Raw *x, const Place &place, bool takes, u32x4 (&raw)[CHUNKS])
 {
-    if (held >= RUN) {
-        typename T::Raw raw[RUN];
-        __builtin_memcpy(raw, x, sizeof raw);
 #pragma unroll
-        for (int j = 0; j < RUN; ++j)
-            v[j] = T::get(raw[j]);
-    } else {
+    for (int i = 0; i < CHUNKS; ++i) {
+        const int held = place.held(i);
+        const typename T::Raw *p = x + place.first + i * place.step;
+        raw[i] = u32x4{T::kNoValue, T::kNoValue, T::kNoValue, T::kNoValue};
+        if (takes && held >= T::kRun) {
+            raw[i] = load_run<T>(p);
+        } else if (takes && held > 0) {
+            float v[T::kRun];
 #pragma unroll
-        for (int j = 0; j < RUN; ++j)
-            v[j] = j < held ? T::get(x[j]) : -INFINITY;
+            for (int j = 0; j < T::kRun; ++j)
+                v[j] = j < held ? T::get(p[j]) : -INFINITY;
+            raw[i] = T::pack(v);
+        }
     }
 }
 
-// Logits become probabilities; returns logsumexp.  A token of -infinity has none: NaN.
-template <int RUN>
-__device__ __forceinline__ float softmax(float (&v)[RUN], int lanes)
+// Probabilities of a token; returns logsumexp.  A token of -infinity has none: NaN.
+template <typename T, int CHUNKS>
+__device__ __forceinline__ float softmax(const u32x4 (&raw)[CHUNKS], int lanes, float (&p)[CHUNKS][T::kRun])
 {
-    float m = v[0];
+    float m = -INFINITY, s = 0.0f;
 #pragma unroll
-    for (int j = 1; j < RUN; ++j)
-        m = fmaxf(m, v[j]);
-    m = spread_max(m, lanes);
-    float s = 0.0f;
+    for (int i = 0; i < CHUNKS; ++i) {
+        T::unpack(raw[i], p[i]);
 #pragma unroll
-    for (int j = 0; j < RUN; ++j) {
-        v[j] = exp2_fast((v[j] - m) * kLog2e);
-        s += v[j];
+        for (int j = 0; j < T::kRun; ++j)
+            m = fmaxf(m, p[i][j]);
     }
-    s = spread_sum(s, lanes);
+    m = token_max(m, lanes);
+#pragma unroll
+    for (int i = 0; i < CHUNKS; ++i)
+#pragma unroll
+        for (int j = 0; j < T::kRun; ++j) {
+            p[i][j] = exp2_fast((p[i][j] - m) * kLog2e);
+            s += p[i][j];
+        }
+    s = token_sum(s, lanes);
     const float inv = 1.0f / s;
 #pragma unroll
-    for (int j = 0; j < RUN; ++j)
-        v[j] *= inv;
+    for (int i = 0; i < CHUNKS; ++i)
+#pragma unroll
+        for (int j = 0; j < T::kRun; ++j)
+            p[i][j] *= inv;
     return m + logf(s);
 }
 
-template <typename T, int RUN>
+// Joins the parts of kJoinColumns experts of a group: counts, the gradient's factors, this tile's part of the loss.  The tile that comes
+// last adds up the parts of the loss, in their order.
+template <int THREADS>
+__device__ __forceinline__ void join(const Balance &a, int64_t group, int tile, double *room, double (*sums)[kJoinColumns])
+{
+    const lpmm_balance_call &c = a.c;
+    constexpr int kSlices = THREADS / kJoinColumns;
+    const int tid = threadIdx.x, experts = (int)c.experts, column = tid % kJoinColumns, slice = tid / kJoinColumns, e = tile * kJoinColumns + column;
+    const int64_t base = group * a.parts;
+    double square = 0.0, tokens = 0.0;
+    bool wrong = false;
+    for (int64_t p = tid; p < a.parts; p += THREADS) {
+        square += a.square[base + p];
+        const int seen = a.seen[base + p];
+        wrong |= seen < 0;
+        tokens += (double)(seen < 0 ? -1 - seen : seen);
+    }
+    double prob = 0.0;
+    int64_t picked = 0;
+    if (e < experts) {
+        for (int64_t p = slice; p < a.parts; p += 8 * kSlices)
+#pragma unroll
+            for (int j = 0; j < 8; ++j)  // loads that do not wait for each other
+                if (p + j * kSlices < a.parts) {
+                    const int64_t at = (base + p + j * kSlices) * experts + e;
+                    prob += (double)a.prob[at];
+                    picked += a.picked[at];
+                }
+    }
+    square = block_sum_f64<THREADS>(square, room);
+    tokens = block_sum_f64<THREADS>(tokens, room);
+    wrong = __syncthreads_or(wrong);
+    sums[slice][column] = prob;
+    __syncthreads();
+    if (slice == 0) {
+        prob = 0.0;
+        for (int i = 0; i < kSlices; ++i)
+            prob += sums[i][column];
+    }
+    __syncthreads();
+    sums[slice][column] = (double)picked;  // exact
+    __syncthreads();
+    double loss = 0.0;
+    const double per = tokens > 0.0 ? 1.0 / tokens : 0.0;
+    if (slice == 0 && e < experts) {
+        double count = 0.0;
+        for (int i = 0; i < kSlices; ++i)
+            count += sums[i][column];
+        const double share = c.picks > 0 ? (double)c.weight * experts * per * per / (double)c.picks : 0.0;
+        c.counts[group * experts + e] = (int64_t)count;
+        c.factors[group * (experts + 2) + e] = wrong ? NAN : (float)(share * count / (double)c.groups);
+        loss = share * count * prob;
+    }
+    loss = block_sum_f64<THREADS>(loss, room);
+    const int64_t all = c.groups * a.tiles;
+    __shared__ bool last;
+    if (tid == 0) {
+        if (tile == 0) {
+            c.factors[group * (experts + 2) + experts] = (float)(2.0 * (double)c.z_weight * per / (double)c.groups);
+            c.factors[group * (experts + 2) + experts + 1] = 0.0f;
+            loss = wrong ? NAN : loss + (double)c.z_weight * square * per;
+        }
+        last = true;
+        if (all == 1) {
+            c.loss[0] = (float)loss;
+            last = false;
+        } else {
+            a.loss_part[group * a.tiles + tile] = loss;
+            __threadfence();
+            last = atomicAdd(a.done, 1u) == (uint32_t)all - 1u;
+            __threadfence();
+        }
+    }
+    __syncthreads();
+    if (!last)
+        return;
+    double s = 0.0;
+    for (int64_t i = tid; i < all; i += THREADS)
+        s += __hip_atomic_load(a.loss_part + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    s = block_sum_f64<THREADS>(s, room);
+    if (tid == 0)
+        c.loss[0] = (float)(s / (double)c.groups);
+}
+
+__global__ __launch_bounds__(kJoinThreads) void balance_join_kernel(Balance a)
+{
+    __shared__ double room[kJoinThreads / kWave];
+    __shared__ double sums[kJoinSlices][kJoinColumns];
+    join<kJoinThreads>(a, blockIdx.x / a.tiles, blockIdx.x % a.tiles, room, sums);
+}
+
+template <typename T, int CHUNKS>
 __global__ __launch_bounds__(kBalThreads) void balance_sums_kernel(Balance a)
 {
-    __shared__ float probs[kBalWaves][LPMM_BALANCE_MOST];
-    __shared__ int counts[LPMM_BALANCE_MOST];
+    constexpr int kRun = T::kRun;
+    __shared__ float probs[kBalWaves][CHUNKS * kLanes * kRun];
+    __shared__ int counts[CHUNKS * kLanes * kRun];
     __shared__ double room[kBalWaves];
     const lpmm_balance_call &c = a.c;
     const int tid = threadIdx.x, experts = (int)c.experts, lane = tid & (kWave - 1);
     const int64_t group = blockIdx.x / a.parts, begin = blockIdx.x % a.parts * a.per;
     const int64_t end = begin + a.per < c.tokens ? begin + a.per : c.tokens;
     const uint8_t *mask = c.mask ? c.mask + group * c.tokens : nullptr;
+    if (blockIdx.x == 0 && tid == 0)
+        *a.done = 0;
+    const Place place = Place::of<T>(a);
+    const int step = kBalThreads / a.lanes;
+    const typename T::Raw *logits = static_cast<const typename T::Raw *>(c.logits) + group * c.outer_stride;
+    auto takes = [&](int64_t n) { return n < end && (!mask || mask[n]); };
+    u32x4 raw[CHUNKS];
+    bool now = takes(begin + tid / a.lanes);
+    load_logits<T, CHUNKS>(logits + (begin + tid / a.lanes) * c.inner_stride, place, now, raw);
+
     for (int e = tid; e < experts; e += kBalThreads)
         counts[e] = 0;
     __syncthreads();
     bool wrong = false;
-    for (int64_t i = begin * c.picks + tid; i < end * c.picks; i += kBalThreads) {
-        if (mask && !mask[i / c.picks])
+    const uint32_t picks = (uint32_t)c.picks;  // tokens * picks fit 31 bits
+    for (uint32_t i = (uint32_t)begin * picks + tid; begin < end && i < (uint32_t)end * picks; i += kBalThreads) {
+        if (mask && !mask[i / picks])
             continue;
-        const int64_t at = group * c.tokens * c.picks + i;
+        const int64_t at = group * c.tokens * picks + i;
         const int64_t id = c.id_bits == 64 ? static_cast<const int64_t *>(c.ids)[at] : static_cast<const int32_t *>(c.ids)[at];
         if (id >= experts)
             wrong = true;
         else if (id >= 0)
             atomicAdd(&counts[id], 1);
     }
-    // the lane's first expert, and how many experts its run holds
-    const int first = (lane & (a.lanes - 1)) * RUN, held = experts - first;
-    float sum[RUN] = {};
+    float sum[CHUNKS][kRun] = {};
     double square = 0.0;
     int seen = 0;
-    const int step = kBalThreads / a.lanes;
     for (int64_t n0 = begin; n0 < end; n0 += step) {  // the waves leave together: lanes exchange values
-        const int64_t n = n0 + tid / a.lanes;
-        const bool takes = n < end && (!mask || mask[n]);
-        float v[RUN];
-        load_logits<T, RUN>(static_cast<const typename T::Raw *>(c.logits) + group * c.outer_stride + n * c.inner_stride + first, takes ? held : 0, v);
-        const float lse = softmax<RUN>(v, a.lanes);
-        if (!takes)
+        float p[CHUNKS][kRun];
+        const float lse = softmax<T, CHUNKS>(raw, a.lanes, p);
+        const bool taken = now;
+        const int64_t next = n0 + step + tid / a.lanes;
+        now = takes(next);
+        load_logits<T, CHUNKS>(logits + next * c.inner_stride, place, now, raw);
+        if (!taken)
             continue;
 #pragma unroll
-        for (int j = 0; j < RUN; ++j)
-            sum[j] += v[j];
-        if (first == 0) {
+        for (int i = 0; i < CHUNKS; ++i)
+#pragma unroll
+            for (int j = 0; j < kRun; ++j)
+                sum[i][j] += p[i][j];
+        if (place.first == 0) {
             square += (double)lse * (double)lse;
             ++seen;
         }
     }
 #pragma unroll
-    for (int j = 0; j < RUN; ++j) {
-        for (int o = a.lanes; o < kWave; o <<= 1)
-            sum[j] += __shfl_xor(sum[j], o, kWave);
-        if (lane < a.lanes && j < held)
-            probs[tid / kWave][first + j] = sum[j];
-    }
+    for (int i = 0; i < CHUNKS; ++i)
+#pragma unroll
+        for (int j = 0; j < kRun; ++j) {
+            for (int o = a.lanes; o < kWave; o <<= 1)
+                sum[i][j] += __shfl_xor(sum[i][j], o, kWave);
+            if (lane < a.lanes && j < place.held(i))
+                probs[tid / kWave][place.first + i * place.step + j] = sum[i][j];
+        }
     __syncthreads();
     for (int e = tid; e < experts; e += kBalThreads) {
         float s = probs[0][e];
@@ -170,104 +311,76 @@ __global__ __launch_bounds__(kBalThreads) void balance_sums_kernel(Balance a)
         a.square[blockIdx.x] = square;
         a.seen[blockIdx.x] = any_wrong ? -1 - all : all;
     }
-}
-
-// One workgroup a group: joins the parts, writes counts, the gradient's factors and the group's loss.
-__global__ __launch_bounds__(kBalThreads) void balance_join_kernel(Balance a)
-{
-    __shared__ double room[kBalWaves];
-    const lpmm_balance_call &c = a.c;
-    const int64_t group = blockIdx.x, base = group * a.parts;
-    const int experts = (int)c.experts;
-    double square = 0.0, tokens = 0.0;
-    bool wrong = false;
-    for (int64_t p = threadIdx.x; p < a.parts; p += kBalThreads) {
-        square += a.square[base + p];
-        const int seen = a.seen[base + p];
-        wrong |= seen < 0;
-        tokens += (double)(seen < 0 ? -1 - seen : seen);
-    }
-    wrong = __syncthreads_or(wrong);
-    square = block_sum_f64<kBalThreads>(square, room);
-    tokens = block_sum_f64<kBalThreads>(tokens, room);
-    const double per = tokens > 0.0 ? 1.0 / tokens : 0.0;
-    const double share = c.picks > 0 ? (double)c.weight * experts * per * per / (double)c.picks : 0.0;
-    float *factors = c.factors + group * (experts + 2);
-    double loss = 0.0;
-    for (int e = threadIdx.x; e < experts; e += kBalThreads) {
-        double prob = 0.0;
-        int64_t picked = 0;
-        for (int64_t p = 0; p < a.parts; ++p) {
-            prob += (double)a.prob[(base + p) * experts + e];
-            picked += a.picked[(base + p) * experts + e];
+    if (gridDim.x == 1) {
+        __shared__ double sums[kBalThreads / kJoinColumns][kJoinColumns];
+        __syncthreads();
+        for (int tile = 0; tile < a.tiles; ++tile) {
+            join<kBalThreads>(a, 0, tile, room, sums);
+            __syncthreads();
         }
-        c.counts[group * experts + e] = picked;
-        factors[e] = wrong ? NAN : (float)(share * (double)picked / (double)c.groups);
-        loss += share * (double)picked * prob;
-    }
-    loss = block_sum_f64<kBalThreads>(loss, room);
-    if (threadIdx.x == 0) {
-        factors[experts] = (float)(2.0 * (double)c.z_weight * per / (double)c.groups);
-        factors[experts + 1] = 0.0f;
-        loss = wrong ? NAN : loss + (double)c.z_weight * square * per;
-        if (c.groups == 1)
-            c.loss[0] = (float)loss;
-        else
-            a.group_loss[group] = loss;
     }
 }
 
-__global__ __launch_bounds__(kBalThreads) void balance_loss_kernel(const double *group_loss, int64_t groups, float *loss)
-{
-    __shared__ double room[kBalWaves];
-    double s = 0.0;
-    for (int64_t g = threadIdx.x; g < groups; g += kBalThreads)
-        s += group_loss[g];
-    s = block_sum_f64<kBalThreads>(s, room);
-    if (threadIdx.x == 0)
-        loss[0] = groups > 0 ? (float)(s / (double)groups) : 0.0f;
-}
+// No groups: the loss is 0.
+__global__ void balance_none_kernel(float *loss) { loss[0] = 0.0f; }
 
-template <typename T, int RUN>
+template <typename T, int CHUNKS>
 __global__ __launch_bounds__(kBalThreads) void balance_grad_kernel(Balance a)
 {
+    constexpr int kRun = T::kRun;
     const lpmm_balance_call &c = a.c;
-    const int tid = threadIdx.x, experts = (int)c.experts, lane = tid & (kWave - 1);
+    const int tid = threadIdx.x, experts = (int)c.experts;
     const int64_t group = blockIdx.x / a.parts, begin = blockIdx.x % a.parts * a.per;
     const int64_t end = begin + a.per < c.tokens ? begin + a.per : c.tokens;
     const uint8_t *mask = c.mask ? c.mask + group * c.tokens : nullptr;
-    const int first = (lane & (a.lanes - 1)) * RUN, held = experts - first;
+    const Place place = Place::of<T>(a);
+    const int step = kBalThreads / a.lanes;
+    const typename T::Raw *logits = static_cast<const typename T::Raw *>(c.logits) + group * c.outer_stride;
+    typename T::Raw *grad = static_cast<typename T::Raw *>(c.grad) + group * c.tokens * experts;
+    auto takes = [&](int64_t n) { return n < end && (!mask || mask[n]); };
+    u32x4 raw[CHUNKS];
+    bool now = takes(begin + tid / a.lanes);
+    load_logits<T, CHUNKS>(logits + (begin + tid / a.lanes) * c.inner_stride, place, now, raw);
     const float *factors = c.factors + group * (experts + 2);
     const float scale = a.grad_loss[0], h = factors[experts];
-    float f[RUN];
+    float f[CHUNKS][kRun];
 #pragma unroll
-    for (int j = 0; j < RUN; ++j)
-        f[j] = j < held ? factors[first + j] : 0.0f;
-    const int step = kBalThreads / a.lanes;
+    for (int i = 0; i < CHUNKS; ++i)
+#pragma unroll
+        for (int j = 0; j < kRun; ++j)
+            f[i][j] = j < place.held(i) ? factors[place.first + i * place.step + j] : 0.0f;
     for (int64_t n0 = begin; n0 < end; n0 += step) {
-        const int64_t n = n0 + tid / a.lanes;
-        const bool takes = n < end && (!mask || mask[n]);
-        float v[RUN];
-        load_logits<T, RUN>(static_cast<const typename T::Raw *>(c.logits) + group * c.outer_stride + n * c.inner_stride + first, takes ? held : 0, v);
-        const float lse = softmax<RUN>(v, a.lanes);
+        float p[CHUNKS][kRun];
+        const float lse = softmax<T, CHUNKS>(raw, a.lanes, p);
+        const bool taken = now;
+        const int64_t n = n0 + tid / a.lanes, next = n + step;
+        now = takes(next);
+        load_logits<T, CHUNKS>(logits + next * c.inner_stride, place, now, raw);
         float dot = 0.0f;
 #pragma unroll
-        for (int j = 0; j < RUN; ++j)
-            dot += f[j] * v[j];
-        dot = spread_sum(dot, a.lanes);
+        for (int i = 0; i < CHUNKS; ++i)
+#pragma unroll
+            for (int j = 0; j < kRun; ++j)
+                dot += f[i][j] * p[i][j];
+        dot = token_sum(dot, a.lanes);
         if (n >= end)
             continue;
-        typename T::Raw out[RUN];
+        const float more = h != 0.0f ? h * lse : 0.0f;
 #pragma unroll
-        for (int j = 0; j < RUN; ++j)
-            out[j] = T::put(takes ? scale * (v[j] * ((f[j] - dot) + (h != 0.0f ? h * lse : 0.0f))) : 0.0f);
-        typename T::Raw *to = static_cast<typename T::Raw *>(c.grad) + (group * c.tokens + n) * experts + first;
-        if (held >= RUN)
-            __builtin_memcpy(to, out, sizeof out);
-        else
-            for (int j = 0; j < RUN; ++j)
-                if (j < held)
-                    to[j] = out[j];
+        for (int i = 0; i < CHUNKS; ++i) {
+            const int held = place.held(i);
+            typename T::Raw *to = grad + n * experts + place.first + i * place.step;
+#pragma unroll
+            for (int j = 0; j < kRun; ++j)
+                p[i][j] = taken ? scale * (p[i][j] * ((f[i][j] - dot) + more)) : 0.0f;
+            if (held >= kRun)
+                store_run<T>(to, T::pack(p[i]));
+            else
+#pragma unroll
+                for (int j = 0; j < kRun; ++j)
+                    if (j < held)
+                        to[j] = T::put(p[i][j]);
+        }
     }
 }
 
@@ -276,7 +389,7 @@ int check_call(const lpmm_balance_call &c)
     if (c.type < LPMM_TYPE_F32 || c.type > LPMM_TYPE_BF16 || (c.id_bits != 32 && c.id_bits != 64) || !isfinite(c.weight) || !isfinite(c.z_weight))
         return LPMM_ERR_ARG;
     if (c.experts < 1 || c.experts > LPMM_BALANCE_MOST || c.picks < 0 || c.picks > c.experts || c.groups < 0 || c.groups > (int64_t)1 << 24 ||
-        c.tokens < 0 || c.tokens > INT32_MAX || c.tokens * (c.picks > 0 ? c.picks : 1) > INT32_MAX || c.outer_stride < 0 || c.inner_stride < 0)
+        c.tokens < 0 || c.tokens > INT32_MAX || c.tokens * (c.picks > 0 ? c.picks : 1) > INT32_MAX || c.groups * c.tokens > INT32_MAX || c.outer_stride < 0 || c.inner_stride < 0)
         return LPMM_ERR_SIZE;
     LPMM_REQUIRE_ALIGN(c.factors, 4);
     if (c.groups == 0)
@@ -289,45 +402,44 @@ int check_call(const lpmm_balance_call &c)
     return LPMM_OK;
 }
 
-Balance arguments(const lpmm_balance_call &c)
-{
-    Balance a = {};
-    a.c = c;
-    const Split s = split(c.groups < 1 ? 1 : c.groups, c.tokens);
-    a.parts = s.parts;
-    a.per = s.per;
-    return a;
-}
-
-template <typename T, int RUN>
+template <typename T, int CHUNKS>
 void launch(Balance a, bool grad, hipStream_t stream)
 {
     a.lanes = 1;
-    while (a.lanes * RUN < a.c.experts)
+    while (a.lanes < kLanes && a.lanes * T::kRun < a.c.experts)
         a.lanes *= 2;
-    const dim3 grid((unsigned)(a.c.groups * a.parts));
-    if (grad)
-        balance_grad_kernel<T, RUN><<<grid, kBalThreads, 0, stream>>>(a);
-    else
-        balance_sums_kernel<T, RUN><<<grid, kBalThreads, 0, stream>>>(a);
+    if (grad) {  // two turns to a workgroup: the second's logits are on their way while the first is computed
+        a.per = 2 * (kBalThreads / a.lanes);
+        a.parts = (a.c.tokens + a.per - 1) / a.per;
+        balance_grad_kernel<T, CHUNKS><<<(unsigned)(a.c.groups * a.parts), kBalThreads, 0, stream>>>(a);
+    } else {
+        balance_sums_kernel<T, CHUNKS><<<(unsigned)(a.c.groups * a.parts), kBalThreads, 0, stream>>>(a);
+    }
 }
 
-template <int RUN>
+template <typename T>
 void launch_type(const Balance &a, bool grad, hipStream_t stream)
 {
-    switch (a.c.type) {
-    case LPMM_TYPE_F32: return launch<F32, RUN>(a, grad, stream);
-    case LPMM_TYPE_F16: return launch<F16, RUN>(a, grad, stream);
-    default: return launch<BF16, RUN>(a, grad, stream);
-    }
+    const int64_t chunks = (a.c.experts + kLanes * T::kRun - 1) / (kLanes * T::kRun);
+    if (chunks <= 1)
+        return launch<T, 1>(a, grad, stream);
+    if (chunks <= 2)
+        return launch<T, 2>(a, grad, stream);
+    if (chunks <= 4)
+        return launch<T, 4>(a, grad, stream);
+    if (T::kRun == 8 || chunks <= 8)
+        return launch<T, 8>(a, grad, stream);
+    if constexpr (T::kRun == 4)
+        launch<T, 16>(a, grad, stream);
 }
 
 void launch_tokens(const Balance &a, bool grad, hipStream_t stream)
 {
-    if (a.c.experts <= 4 * kWave)
-        launch_type<4>(a, grad, stream);
-    else
-        launch_type<16>(a, grad, stream);
+    switch (a.c.type) {
+    case LPMM_TYPE_F32: return launch_type<F32>(a, grad, stream);
+    case LPMM_TYPE_F16: return launch_type<F16>(a, grad, stream);
+    default: return launch_type<BF16>(a, grad, stream);
+    }
 }
 
 }  // namespace
@@ -337,8 +449,9 @@ extern "C" int64_t lpmm_balance_work_bytes(int64_t groups, int64_t tokens, int64
 {
     if (groups < 1 || tokens < 0 || experts < 1)
         return 0;
-    const int64_t rows = groups * lpmm::split(groups, tokens).parts;
-    return rows * 8 + groups * 8 + (rows * experts * 2 + rows) * 4;
+    const lpmm::Split s = lpmm::split(groups, tokens, experts);
+    const int64_t rows = groups * s.parts;
+    return rows * 8 + groups * s.tiles * 8 + (rows * experts * 2 + rows + 1) * 4;
 }
 
 extern "C" int lpmm_balance_loss(const lpmm_balance_call *call, void *stream)
@@ -360,19 +473,26 @@ extern "C" int lpmm_balance_loss(const lpmm_balance_call *call, void *stream)
     LPMM_REQUIRE_ALIGN(c.counts, 8);
     LPMM_REQUIRE_ALIGN(c.work, 8);
     hipStream_t s = static_cast<hipStream_t>(stream);
-    Balance a = arguments(c);
-    if (c.groups > 0) {
-        const int64_t rows = c.groups * a.parts;
-        a.square = static_cast<double *>(c.work);
-        a.group_loss = a.square + rows;
-        a.prob = reinterpret_cast<float *>(a.group_loss + c.groups);
-        a.picked = reinterpret_cast<int32_t *>(a.prob + rows * c.experts);
-        a.seen = a.picked + rows * c.experts;
-        launch_tokens(a, false, s);
-        balance_join_kernel<<<(unsigned)c.groups, kBalThreads, 0, s>>>(a);
+    if (c.groups == 0) {
+        balance_none_kernel<<<1, 1, 0, s>>>(c.loss);
+        return launch_status();
     }
-    if (c.groups != 1)
-        balance_loss_kernel<<<1, kBalThreads, 0, s>>>(a.group_loss, c.groups, c.loss);
+    const Split cut = split(c.groups, c.tokens, c.experts);
+    const int64_t rows = c.groups * cut.parts;
+    Balance a = {};
+    a.c = c;
+    a.parts = cut.parts;
+    a.per = cut.per;
+    a.tiles = (int)cut.tiles;
+    a.square = static_cast<double *>(c.work);
+    a.loss_part = a.square + rows;
+    a.prob = reinterpret_cast<float *>(a.loss_part + c.groups * cut.tiles);
+    a.picked = reinterpret_cast<int32_t *>(a.prob + rows * c.experts);
+    a.seen = a.picked + rows * c.experts;
+    a.done = reinterpret_cast<uint32_t *>(a.seen + rows);
+    launch_tokens(a, false, s);
+    if (rows > 1)
+        balance_join_kernel<<<(unsigned)(c.groups * cut.tiles), kJoinThreads, 0, s>>>(a);
     return launch_status();
 }
 
@@ -389,7 +509,8 @@ extern "C" int lpmm_balance_loss_grad(const lpmm_balance_call *call, const float
     LPMM_REQUIRE_PTR(c.grad);
     LPMM_REQUIRE_ALIGN(grad_loss, 4);
     LPMM_REQUIRE_ALIGN(c.grad, c.type == LPMM_TYPE_F32 ? 4 : 2);
-    Balance a = arguments(c);
+    Balance a = {};
+    a.c = c;
     a.grad_loss = grad_loss;
     launch_tokens(a, true, static_cast<hipStream_t>(stream));
     return launch_status();

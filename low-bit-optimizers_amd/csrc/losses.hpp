@@ -105,6 +105,12 @@ __device__ __forceinline__ u32x4 load_run_once(const typename T::Raw *p)
 }
 
 template <typename T>
+__device__ __forceinline__ void store_run(typename T::Raw *p, u32x4 r)
+{
+    *reinterpret_cast<u32x4_any *>(p) = r;
+}
+
+template <typename T>
 __device__ __forceinline__ void store_run_once(typename T::Raw *p, u32x4 r)
 {
     __builtin_nontemporal_store(r, reinterpret_cast<u32x4_any *>(p));
