@@ -22,6 +22,7 @@ struct Distill {
     int64_t grad_loss_stride;
     int made;        // the gradient call: grad holds what belongs to grad_loss == 1
     int with_label;  // labels that have a weight
+    int group_shift;  // teacher_group = 2^group_shift, or -1
     int far;         // the logits are more than the last-level cache holds
     float each;      // weight of a row in the reduced loss where no `share` says it
 };
@@ -70,25 +71,32 @@ __device__ __forceinline__ const typename T::Raw *row_of(const lpmm_distill_call
 // One entry of the teacher, as the thread that has it keeps it.  What is loaded stays as it is stored until it is used: whoever converts
 // waits, and the row's loads have to be on their way by then.
 struct Entry {
-    int64_t id;         // -1: none
+    uint32_t id_low, id_high;
     uint32_t value, x;  // the teacher's value and the student's logit, as stored
     float scale;        // of a value in codes
     float t;
 
-    __device__ __forceinline__ void load(const lpmm_distill_call &c, int64_t at)
+    __device__ __forceinline__ void load(const Distill &a, int64_t at)
     {
-        if (c.id_bits == 64)
-            id = static_cast<const int64_t *>(c.ids)[at];
-        else
-            id = static_cast<const int32_t *>(c.ids)[at];
+        const lpmm_distill_call &c = a.c;
+        if (c.id_bits == 64) {
+            const uint2 id = static_cast<const uint2 *>(c.ids)[at];
+            id_low = id.x, id_high = id.y;
+        } else {
+            id_low = static_cast<const uint32_t *>(c.ids)[at];
+        }
         if (c.teacher_type == LPMM_TYPE_F32) {
             value = static_cast<const uint32_t *>(c.teacher)[at];
         } else if (c.teacher_type != LPMM_TYPE_CODES) {
             value = static_cast<const uint16_t *>(c.teacher)[at];
         } else {
             value = static_cast<const uint8_t *>(c.teacher)[c.teacher_bits == 4 ? at >> 1 : at];
-            scale = c.teacher_scale[at / c.teacher_group];
+            scale = c.teacher_scale[a.group_shift >= 0 ? at >> a.group_shift : at / c.teacher_group];
         }
+    }
+    __device__ __forceinline__ int64_t id(const lpmm_distill_call &c) const
+    {
+        return c.id_bits == 64 ? (int64_t)((uint64_t)id_high << 32 | id_low) : (int64_t)(int32_t)id_low;
     }
     __device__ __forceinline__ float value_of(const lpmm_distill_call &c, int64_t at) const
     {
@@ -304,9 +312,8 @@ __global__ __launch_bounds__(THREADS, WAVES) void distill_kernel(Distill a)
     // everything that the row needs is asked for before anything is looked at
     Entry entry;  // one to a thread: topk is at most THREADS
     const bool has_entry = (int)tid < topk;
-    entry.id = -1;
     if (has_entry)
-        entry.load(c, row * topk + tid);
+        entry.load(a, row * topk + tid);
     const bool label_wrong = c.labels && (label < 0 || label >= c.vocab), has_label = a.with_label && !label_wrong;
     const uint32_t label_bits = load_bits<T>(x + (has_label ? label : 0)), alone_bits = load_bits<T>(x + (single < vocab ? single : 0));
     u32x4 held[RUNS > 0 ? RUNS : 1];
@@ -333,11 +340,14 @@ __global__ __launch_bounds__(THREADS, WAVES) void distill_kernel(Distill a)
     }
     bool wrong = label_wrong;
     const bool has_entries = (int)(wave * kWave) < topk;
+    int64_t id = -1;  // none
     if (has_entries) {
-        wrong |= entry.id >= c.vocab;
-        if (entry.id >= c.vocab)
-            entry.id = -1;
-        entry.x = load_bits<T>(x + (entry.id >= 0 ? entry.id : 0));
+        if (has_entry)
+            id = entry.id(c);
+        wrong |= id >= c.vocab;
+        if (id >= c.vocab)
+            id = -1;
+        entry.x = load_bits<T>(x + (id >= 0 ? id : 0));
     }
     // each run of the thread, from where it is held; or read again, for what is seldom done (and for rows that are not held)
     auto read_runs = [&](auto &&body) {
@@ -365,10 +375,10 @@ __global__ __launch_bounds__(THREADS, WAVES) void distill_kernel(Distill a)
     auto look = [&] {  // the wave's part of the teacher's softmax
         if (!has_entries)
             return;
-        entry.t = entry.id >= 0 ? entry.value_of(c, row * topk + tid) : -INFINITY;
+        entry.t = id >= 0 ? entry.value_of(c, row * topk + tid) : -INFINITY;
         wrong |= !(entry.t < INFINITY);
         if (has_entry)
-            ids[tid] = (int)entry.id;
+            ids[tid] = (int)id;
         top = wave_max(entry.t);
         total = wave_sum(top > -INFINITY ? expf((entry.t - top) * inv_t) : 0.0f);
     };
@@ -503,8 +513,8 @@ __global__ __launch_bounds__(THREADS, WAVES) void distill_kernel(Distill a)
         return;
     // the listed entries and the label again, with what they take off: one thread for each id
     float off;
-    if (has_entry && entry.id >= 0 && takes_off(ids, part, listed, tid, off))
-        grad[entry.id] = T::put(value_of(from_bits<T>(entry.x)) - off);
+    if (id >= 0 && takes_off(ids, part, listed, tid, off))
+        grad[id] = T::put(value_of(from_bits<T>(entry.x)) - off);
     if (tid == 0 && ids[topk] >= 0 && takes_off(ids, part, listed, topk, off))
         grad[label] = T::put(value_of(from_bits<T>(label_bits)) - off);
 }
@@ -580,6 +590,9 @@ Distill arguments(const lpmm_distill_call &c)
     if (c.teacher_weight == 0.0f)
         a.c.topk = 0;  // a term without weight is not looked at
     a.with_label = c.labels && c.label_weight != 0.0f;
+    a.group_shift = -1;
+    if (c.teacher_group > 0 && (c.teacher_group & (c.teacher_group - 1)) == 0)
+        a.group_shift = __builtin_ctzll((unsigned long long)c.teacher_group);
     a.far = c.rows * c.vocab * (c.type == LPMM_TYPE_F32 ? 4 : 2) > kLastLevel;
     a.each = c.reduction == LPMM_REDUCE_MEAN && !c.labels ? (float)(1.0 / (double)c.rows) : 1.0f;
     return a;
