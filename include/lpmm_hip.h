@@ -850,7 +850,7 @@ typedef struct lpmm_distill_call {
     float *row_loss;            /* [rows]: the loss of each row (written in every reduction) */
     float *row_stats;           /* [rows][4], 16-byte aligned: what the gradient call needs of each row; NULL: not kept */
     float *loss;                /* [1]: the reduced loss; NULL with LPMM_REDUCE_NONE */
-    float *share;               /* [1]: work of the mean with labels, kept for the gradient call: 1 / rows that count */
+    float *share;               /* [1]: work of the mean with labels, kept for the gradient call */
     void *grad;                 /* [rows][vocab] of `type`: the reduced loss's gradient, from the same pass; NULL: not wanted */
     int64_t rows, vocab, topk;  /* rows: 0 .. 2^31 - 1; vocab: 1 .. 2^31 - 1; topk: 0 .. LPMM_DISTILL_MOST */
     int64_t inner, outer_stride, inner_stride;

@@ -16,8 +16,17 @@ namespace {
 
 constexpr int64_t kLastLevel = (int64_t)256 << 20;  // bytes of the memory-side cache
 
+// Where the weight 1 / (rows that count) of the mean with labels comes from.
+enum Shared {
+    kNoShare,    // not that mean
+    kCounted,    // a kernel before: c.share
+    kCountHere,  // few rows: every workgroup counts them, a microsecond each at once, for a launch less
+};
+constexpr int64_t kFewRows = 256;  // at most a workgroup's threads
+
 struct Distill {
     lpmm_distill_call c;
+    int shared;
     const float *grad_loss;  // the gradient call: not NULL
     int64_t grad_loss_stride;
     int made;        // the gradient call: grad holds what belongs to grad_loss == 1
@@ -60,6 +69,13 @@ __device__ __forceinline__ void shifts(float max, float c, Shift &t, Shift &one)
     one = KIND == kTwo ? Shift::of<T>(max, kLog2e) : KIND == kSquare ? Shift{max, kLog2e, 2.0f * t.m} : t;
     if (KIND == kTwo && !(t.one_step() && one.one_step()))
         t.m = one.m = NAN;
+}
+
+// 1 / rows that count, of at most as many rows as the workgroup has threads.
+__device__ __forceinline__ double share_of_few(const int64_t *labels, int64_t rows, int64_t ignore)
+{
+    const int n = __syncthreads_count((int64_t)threadIdx.x < rows && labels[threadIdx.x] != ignore);
+    return n > 0 ? 1.0 / n : 0.0;
 }
 
 template <typename T>
@@ -281,12 +297,15 @@ __global__ __launch_bounds__(THREADS, WAVES) void distill_kernel(Distill a)
     const int64_t row = blockIdx.x;
     float scale = a.each;
     if constexpr (AGAIN) {
-        scale *= a.grad_loss[row * a.grad_loss_stride];
-        if (a.made && scale == a.each)  // times 1
+        const float g = a.grad_loss[row * a.grad_loss_stride];
+        if (a.made && g == 1.0f)
             return;
+        scale *= g;
     }
-    if (c.reduction == LPMM_REDUCE_MEAN && c.labels)
+    if (a.shared == kCounted)
         scale *= c.share[0];
+    else if (a.shared == kCountHere)
+        scale *= (float)share_of_few(c.labels, c.rows, c.ignore_index);
     const int topk = (int)c.topk, listed = topk + 1, places = (listed + 3) & ~3;
     int *ids = entries;
     float *part = reinterpret_cast<float *>(entries + places);
@@ -535,18 +554,21 @@ __global__ __launch_bounds__(kSumThreads) void distill_share_kernel(const int64_
         share[0] = all > 0.0 ? (float)(1.0 / all) : 0.0f;
 }
 
-// Sum of the rows' losses in double, in a fixed order, times `each` or *share.
-__global__ __launch_bounds__(kSumThreads) void distill_sum_kernel(const float *row_loss, int64_t rows, const float *share, double each, float *loss)
+// Sum of the rows' losses in double, in a fixed order, times their weight.
+__global__ __launch_bounds__(kSumThreads) void distill_sum_kernel(Distill a, double each)
 {
     __shared__ double room[kSumThreads / kWave];
+    const lpmm_distill_call &c = a.c;
+    if (a.shared == kCountHere)
+        each = share_of_few(c.labels, c.rows, c.ignore_index);
     double s = 0.0;
-    for (int64_t i = threadIdx.x; i < rows; i += 8 * kSumThreads)
+    for (int64_t i = threadIdx.x; i < c.rows; i += 8 * kSumThreads)
 #pragma unroll
         for (int j = 0; j < 8; ++j)
-            s += i + j * kSumThreads < rows ? (double)row_loss[i + j * kSumThreads] : 0.0;
+            s += i + j * kSumThreads < c.rows ? (double)c.row_loss[i + j * kSumThreads] : 0.0;
     s = block_sum_f64<kSumThreads>(s, room);
     if (threadIdx.x == 0)
-        loss[0] = (float)(s * (share ? (double)share[0] : each));
+        c.loss[0] = (float)(s * (a.shared == kCounted ? (double)c.share[0] : each));
 }
 
 int check_call(const lpmm_distill_call &c)
@@ -590,6 +612,8 @@ Distill arguments(const lpmm_distill_call &c)
     if (c.teacher_weight == 0.0f)
         a.c.topk = 0;  // a term without weight is not looked at
     a.with_label = c.labels && c.label_weight != 0.0f;
+    if (c.reduction == LPMM_REDUCE_MEAN && c.labels)
+        a.shared = c.rows <= kFewRows ? kCountHere : kCounted;
     a.group_shift = -1;
     if (c.teacher_group > 0 && (c.teacher_group & (c.teacher_group - 1)) == 0)
         a.group_shift = __builtin_ctzll((unsigned long long)c.teacher_group);
@@ -617,7 +641,7 @@ void launch_kind(const Distill &a, hipStream_t stream)
     // loss and gradient of 1 GB (16 KB rows: 268 MB), us with the neighbouring choices: 8192 values 60 (256 x 8 59, 512 x 8 76), 16384: 107 (512 x 8
     // 111), 32000: 196 (256 x 16 200, 1024 x 7 204), 50257: 204 (1024 x 8 210, 512 x 16 215), 65536: 196 (512 x 16 194, 1024 x 16 234).
     // Fewer rows than compute units: the most threads a row can have.
-    if (a.c.rows < 256) {
+    if (a.c.rows < kFewRows) {
         if (fits(1024, 4))
             return launch<T, KIND, 1024, 4, 4>(a, stream);
     } else {
@@ -678,14 +702,12 @@ extern "C" int lpmm_distill_loss(const lpmm_distill_call *call, void *stream)
     LPMM_REQUIRE_ALIGN(c.grad, c.type == LPMM_TYPE_F32 ? 4 : 2);
     hipStream_t s = static_cast<hipStream_t>(stream);
     const Distill a = arguments(c);
-    const bool shared = c.reduction == LPMM_REDUCE_MEAN && c.labels;
-    if (shared)
+    if (a.shared == kCounted)
         distill_share_kernel<<<1, kSumThreads, 0, s>>>(c.labels, c.rows, c.ignore_index, c.share);
     if (c.rows > 0)
         launch_rows(a, s);
     if (c.reduction != LPMM_REDUCE_NONE)
-        distill_sum_kernel<<<1, kSumThreads, 0, s>>>(c.row_loss, c.rows, shared ? c.share : nullptr,
-                                                     c.reduction == LPMM_REDUCE_MEAN && c.rows > 0 ? 1.0 / (double)c.rows : 1.0, c.loss);
+        distill_sum_kernel<<<1, kSumThreads, 0, s>>>(a, c.reduction == LPMM_REDUCE_MEAN && c.rows > 0 ? 1.0 / (double)c.rows : 1.0);
     return launch_status();
 }
 

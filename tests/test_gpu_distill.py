@@ -68,7 +68,7 @@ def test_numbers_of_entries(topk):
             _check(x, t, ids.int(), y, temperature=3.0, label_weight=1.0, what=f"{topk} of {vocab} with labels")
 
 
-@pytest.mark.parametrize("rows", [0, 1, 2, 5, 64, 300, 2500])
+@pytest.mark.parametrize("rows", [0, 1, 2, 5, 64, 255, 256, 257, 300, 2500])
 @pytest.mark.parametrize("reduction", ["mean", "sum", "none"])
 def test_rows_and_reductions(rows, reduction):
     for dtype in (torch.bfloat16, torch.float16):
