@@ -381,7 +381,9 @@ __global__ __launch_bounds__(THREADS, WAVES) void distill_kernel(Distill a)
                 if (cut.head + i * kStride < cut.end) {
                     const uint32_t at = first + i * kStride;
                     asm volatile("" : "+v"(held[i]));  // unpacked anew each time: the floats of a row do not fit
-                    body(at, at < cut.end ? held[i] : u32x4{T::kNoValue, T::kNoValue, T::kNoValue, T::kNoValue});
+                    if (cut.head + (i + 1) * kStride > cut.end && at >= cut.end)  // no branch that most runs need to look at
+                        held[i] = u32x4{T::kNoValue, T::kNoValue, T::kNoValue, T::kNoValue};
+                    body(at, held[i]);
                 }
         } else {
             read_runs(body);
