@@ -7,8 +7,15 @@
 // constants of the row, less what the few listed entries and the label take off.
 //
 // One workgroup takes a row and holds it in registers, as it came, 16 bytes a run: a row of logits is read once and a row of the gradient written
-// once, with the maximum, the sums and the gradient made from what is held.  The first wave takes the teacher's entries meanwhile.  Rows too long to
-// hold are read twice.
+// once, with the sums and the gradient made from what is held.  Entries are asked for before the row and looked at when it has come.  Rows too
+// long to hold are read twice.
+//
+// Bound by memory: without any exponential the kernel takes as long (8188 x 32000 bf16: 203 us with them, 206 without).  Loss and gradient of that
+// batch, a tenth of its rows left out by their labels, move 1.00 GB in 188 us, 5.3 TB/s, where a copy of 4 GB by the library reaches 4.9; evaluation
+// alone reads 6.2 TB/s.  What a row costs beside its bytes is a chain of some 7 us (label, entries, logits at the entries, two barriers,
+// the last stores), hidden by the other workgroups of a compute unit; rows over 65536 16-bit values leave room for one, and move 4.7 TB/s.
+//
+// The gradient belongs to the loss's own pass because the row is at hand there: 4 bytes a bf16 value where a second pass moves 6.
 #include "losses.hpp"
 
 namespace lpmm {
@@ -26,14 +33,14 @@ constexpr int64_t kFewRows = 256;  // at most a workgroup's threads
 
 struct Distill {
     lpmm_distill_call c;
-    int shared;
     const float *grad_loss;  // the gradient call: not NULL
     int64_t grad_loss_stride;
-    int made;        // the gradient call: grad holds what belongs to grad_loss == 1
-    int with_label;  // labels that have a weight
+    int made;         // the gradient call: grad holds what belongs to grad_loss == 1
+    int shared;       // enum Shared
+    int with_label;   // labels that have a weight
     int group_shift;  // teacher_group = 2^group_shift, or -1
-    int far;         // the logits are more than the last-level cache holds
-    float each;      // weight of a row in the reduced loss where no `share` says it
+    int far;          // the logits are more than the last-level cache holds
+    float each;       // weight of a row in the reduced loss where `shared` does not say it
 };
 
 // Exponentials of a row: exp((x - max) / T), and exp(x - max) for the label's term.
@@ -43,9 +50,9 @@ enum Kind {
     kTwo,
 };
 
-// How exponents of 2 are formed.  16-bit types: fma(x, c, -M) with M = max c, one instruction; what rounding M leaves is the same factor
-// in every exponential of the row and in its sum, so long as it is small, which |M| below 2^20 ensures (2^-4 at most in the exponent).
-// Rows beyond and float32 logits subtract first: a row of the type's lowest values only has a uniform softmax and no overflow.
+// How exponents of 2 are formed: fma(x, c, -M) with M = max c, one instruction; what rounding M leaves is the same factor in every
+// exponential of the row and in its sum, so long as it is small, which |M| below 2^20 ensures (2^-4 at most in the exponent).
+// Rows beyond subtract first: a row of the type's lowest values only has a uniform softmax and no overflow.
 constexpr float kLargeShift = 1048576.0f;
 
 struct Shift {
@@ -54,7 +61,7 @@ struct Shift {
     static __device__ __forceinline__ Shift of(float max, float c)
     {
         const float m = max * c;
-        return {max, c, T::kRun == 8 && fabsf(m) < kLargeShift ? m : NAN};
+        return {max, c, fabsf(m) < kLargeShift ? m : NAN};
     }
     __device__ __forceinline__ bool one_step() const { return m == m; }
     // the exponent, for a few values of a row
@@ -257,24 +264,18 @@ struct Sums {
     float max, sum, sum1;
 };
 
-template <int KIND, bool ONE_STEP>
-__device__ __forceinline__ float from_to(float from, float to, float c)
-{
-    return ONE_STEP ? exp2_fast(from * c - to * c) : exp2_fast((from - to) * c);
-}
-
 // Sums relative to another maximum.
-template <int KIND, bool ONE_STEP>
+template <int KIND>
 __device__ __forceinline__ void rebase(Sums &s, float max, float c)
 {
     if (s.sum == 0.0f)  // nothing yet, whatever its maximum
         return;
-    const float f = from_to<KIND, ONE_STEP>(s.max, max, c);
+    const float f = exp2_fast(s.max * c - max * c);  // of the two shifts as they were rounded
     s.sum *= f;
     if (KIND == kSquare)
         s.sum1 *= f * f;
     if (KIND == kTwo)
-        s.sum1 *= from_to<KIND, ONE_STEP>(s.max, max, kLog2e);
+        s.sum1 *= exp2_fast(s.max * kLog2e - max * kLog2e);
 }
 
 // RUNS runs of 16 bytes in each thread; RUNS = 0: rows of any length, read twice.
@@ -285,7 +286,6 @@ __global__ __launch_bounds__(THREADS, WAVES) void distill_kernel(Distill a)
     using Raw = typename T::Raw;
     constexpr uint32_t kStride = THREADS * T::kRun;
     constexpr int kWaves = THREADS / kWave;
-    constexpr bool kOneStep = T::kRun == 8;
     static_assert(kWaves >= 4 && kWaves <= 16, "lanes_sum");
     struct OfWave {
         float max, sum, sum1, top, total, kd;
@@ -425,13 +425,13 @@ __global__ __launch_bounds__(THREADS, WAVES) void distill_kernel(Distill a)
         Sums s = {none ? 0.0f : m, 0.0f, 0.0f};
         Shift t, one;
         shifts<T, KIND>(s.max, ct, t, one);
-        s.sum = exp2_fast(kOneStep ? fmaf(alone, t.c, -t.m) : (alone - t.max) * t.c);
-        s.sum1 = KIND == kSquare ? s.sum * s.sum : KIND == kTwo ? exp2_fast(kOneStep ? fmaf(alone, one.c, -one.m) : (alone - one.max) * one.c) : 0.0f;
-        runs([&](uint32_t, u32x4 r) { run_sums<T, KIND, kOneStep>(r, t, one, s.sum, s.sum1); });
+        s.sum = exp2_fast(fmaf(alone, t.c, -t.m));
+        s.sum1 = KIND == kSquare ? s.sum * s.sum : KIND == kTwo ? exp2_fast(fmaf(alone, one.c, -one.m)) : 0.0f;
+        runs([&](uint32_t, u32x4 r) { run_sums<T, KIND, true>(r, t, one, s.sum, s.sum1); });
         // s.sum is NaN where t.m is: values too large for one step
         const bool fit = !(none && first < cut.end) && s.sum < 0x1p30f && (KIND != kTwo || s.sum1 < 0x1p30f);
         const float most = wave_max(s.sum == 0.0f ? -INFINITY : s.max);
-        rebase<KIND, kOneStep>(s, most, ct);
+        rebase<KIND>(s, most, ct);
         s.sum = wave_sum(s.sum);
         if (KIND != kOne)
             s.sum1 = wave_sum(s.sum1);
@@ -444,7 +444,7 @@ __global__ __launch_bounds__(THREADS, WAVES) void distill_kernel(Distill a)
         const bool fine = __all(of.fits);
         all.max = lanes_max<kWaves>(of.max);
         s = {of.max, of.sum, of.sum1};
-        rebase<KIND, kOneStep>(s, all.max, ct);
+        rebase<KIND>(s, all.max, ct);
         all.sum = lanes_sum<kWaves>(s.sum);
         all.sum1 = lanes_sum<kWaves>(s.sum1);
         if (!fine || !(all.sum < 0x1p30f)) {  // the largest value first, then differences to it
@@ -461,8 +461,8 @@ __global__ __launch_bounds__(THREADS, WAVES) void distill_kernel(Distill a)
             shifts<T, KIND>(largest, ct, t, one);
             s.sum = exp2_fast(t.of_value(alone));
             s.sum1 = KIND == kSquare ? s.sum * s.sum : KIND == kTwo ? exp2_fast(one.of_value(alone)) : 0.0f;
-            if (kOneStep && t.one_step())
-                read_runs([&](uint32_t, u32x4 r) { run_sums<T, KIND, kOneStep>(r, t, one, s.sum, s.sum1); });
+            if (t.one_step())
+                read_runs([&](uint32_t, u32x4 r) { run_sums<T, KIND, true>(r, t, one, s.sum, s.sum1); });
             else
                 read_runs([&](uint32_t, u32x4 r) { run_sums<T, KIND, false>(r, t, one, s.sum, s.sum1); });
             s.sum = wave_sum(s.sum);
@@ -509,9 +509,9 @@ __global__ __launch_bounds__(THREADS, WAVES) void distill_kernel(Distill a)
         return smooth<KIND>(exp2_fast(t.of_value(v)), KIND == kTwo ? exp2_fast(one.of_value(v)) : 0.0f, f);
     };
     if (grad) {
-        if (!kOneStep || t.one_step())
+        if (!true || t.one_step())
             runs([&](uint32_t at, u32x4 r) {
-                const u32x4 g = run_grad<T, KIND, kOneStep>(r, t, one, f);
+                const u32x4 g = run_grad<T, KIND, true>(r, t, one, f);
                 if (at < cut.end)
                     store_run_once<T>(grad + at, g);
             });
@@ -668,7 +668,7 @@ void launch_type(const Distill &a, hipStream_t stream)
 {
     if (!a.with_label || a.c.temperature == 1.0f)
         return launch_kind<T, kOne>(a, stream);
-    if constexpr (T::kRun == 8)
+    if constexpr (T::kRun == 8)  // float32 rows move twice the bytes for as many exponentials
         if (a.c.temperature == 2.0f)
             return launch_kind<T, kSquare>(a, stream);
     launch_kind<T, kTwo>(a, stream);
