@@ -50,9 +50,11 @@ enum Kind {
     kTwo,
 };
 
-// How exponents of 2 are formed: fma(x, c, -M) with M = max c, one instruction; what rounding M leaves is the same factor in every
-// exponential of the row and in its sum, so long as it is small, which |M| below 2^20 ensures (2^-4 at most in the exponent).
-// Rows beyond subtract first: a row of the type's lowest values only has a uniform softmax and no overflow.
+// How exponents of 2 are formed.  16-bit types: fma(x, c, -M) with M = max c, one instruction; what rounding M leaves is the same factor
+// in every exponential of the row and in its sum, so long as it is small, which |M| below 2^20 ensures (2^-4 at most in the exponent).
+// Rows beyond subtract first: a row of the type's lowest values only has a uniform softmax and no overflow.  So do float32 logits, whose
+// kernels wait for twice the bytes and need the registers (2048 x 32000 at T = 1.5 and a label's term: 185 us, 193 in one step; bf16 rows
+// of 50257 at T = 1 lose 5 % if they subtract).
 constexpr float kLargeShift = 1048576.0f;
 
 struct Shift {
@@ -61,7 +63,7 @@ struct Shift {
     static __device__ __forceinline__ Shift of(float max, float c)
     {
         const float m = max * c;
-        return {max, c, fabsf(m) < kLargeShift ? m : NAN};
+        return {max, c, T::kRun == 8 && fabsf(m) < kLargeShift ? m : NAN};
     }
     __device__ __forceinline__ bool one_step() const { return m == m; }
     // the exponent, for a few values of a row
@@ -264,18 +266,25 @@ struct Sums {
     float max, sum, sum1;
 };
 
+// What exponentials relative to one maximum are worth relative to another; in one step: of the two shifts as they were rounded.
+template <bool ONE_STEP>
+__device__ __forceinline__ float from_to(float from, float to, float c)
+{
+    return ONE_STEP ? exp2_fast(from * c - to * c) : exp2_fast((from - to) * c);
+}
+
 // Sums relative to another maximum.
-template <int KIND>
+template <int KIND, bool ONE_STEP>
 __device__ __forceinline__ void rebase(Sums &s, float max, float c)
 {
     if (s.sum == 0.0f)  // nothing yet, whatever its maximum
         return;
-    const float f = exp2_fast(s.max * c - max * c);  // of the two shifts as they were rounded
+    const float f = from_to<ONE_STEP>(s.max, max, c);
     s.sum *= f;
     if (KIND == kSquare)
         s.sum1 *= f * f;
     if (KIND == kTwo)
-        s.sum1 *= exp2_fast(s.max * kLog2e - max * kLog2e);
+        s.sum1 *= from_to<ONE_STEP>(s.max, max, kLog2e);
 }
 
 // RUNS runs of 16 bytes in each thread; RUNS = 0: rows of any length, read twice.
@@ -286,6 +295,7 @@ __global__ __launch_bounds__(THREADS, WAVES) void distill_kernel(Distill a)
     using Raw = typename T::Raw;
     constexpr uint32_t kStride = THREADS * T::kRun;
     constexpr int kWaves = THREADS / kWave;
+    constexpr bool kOneStep = T::kRun == 8;
     static_assert(kWaves >= 4 && kWaves <= 16, "lanes_sum");
     struct OfWave {
         float max, sum, sum1, top, total, kd;
@@ -425,13 +435,13 @@ __global__ __launch_bounds__(THREADS, WAVES) void distill_kernel(Distill a)
         Sums s = {none ? 0.0f : m, 0.0f, 0.0f};
         Shift t, one;
         shifts<T, KIND>(s.max, ct, t, one);
-        s.sum = exp2_fast(fmaf(alone, t.c, -t.m));
-        s.sum1 = KIND == kSquare ? s.sum * s.sum : KIND == kTwo ? exp2_fast(fmaf(alone, one.c, -one.m)) : 0.0f;
-        runs([&](uint32_t, u32x4 r) { run_sums<T, KIND, true>(r, t, one, s.sum, s.sum1); });
+        s.sum = exp2_fast(kOneStep ? fmaf(alone, t.c, -t.m) : (alone - t.max) * t.c);
+        s.sum1 = KIND == kSquare ? s.sum * s.sum : KIND == kTwo ? exp2_fast(kOneStep ? fmaf(alone, one.c, -one.m) : (alone - one.max) * one.c) : 0.0f;
+        runs([&](uint32_t, u32x4 r) { run_sums<T, KIND, kOneStep>(r, t, one, s.sum, s.sum1); });
         // s.sum is NaN where t.m is: values too large for one step
         const bool fit = !(none && first < cut.end) && s.sum < 0x1p30f && (KIND != kTwo || s.sum1 < 0x1p30f);
         const float most = wave_max(s.sum == 0.0f ? -INFINITY : s.max);
-        rebase<KIND>(s, most, ct);
+        rebase<KIND, kOneStep>(s, most, ct);
         s.sum = wave_sum(s.sum);
         if (KIND != kOne)
             s.sum1 = wave_sum(s.sum1);
@@ -444,7 +454,7 @@ __global__ __launch_bounds__(THREADS, WAVES) void distill_kernel(Distill a)
         const bool fine = __all(of.fits);
         all.max = lanes_max<kWaves>(of.max);
         s = {of.max, of.sum, of.sum1};
-        rebase<KIND>(s, all.max, ct);
+        rebase<KIND, kOneStep>(s, all.max, ct);
         all.sum = lanes_sum<kWaves>(s.sum);
         all.sum1 = lanes_sum<kWaves>(s.sum1);
         if (!fine || !(all.sum < 0x1p30f)) {  // the largest value first, then differences to it
@@ -461,8 +471,8 @@ __global__ __launch_bounds__(THREADS, WAVES) void distill_kernel(Distill a)
             shifts<T, KIND>(largest, ct, t, one);
             s.sum = exp2_fast(t.of_value(alone));
             s.sum1 = KIND == kSquare ? s.sum * s.sum : KIND == kTwo ? exp2_fast(one.of_value(alone)) : 0.0f;
-            if (t.one_step())
-                read_runs([&](uint32_t, u32x4 r) { run_sums<T, KIND, true>(r, t, one, s.sum, s.sum1); });
+            if (kOneStep && t.one_step())
+                read_runs([&](uint32_t, u32x4 r) { run_sums<T, KIND, kOneStep>(r, t, one, s.sum, s.sum1); });
             else
                 read_runs([&](uint32_t, u32x4 r) { run_sums<T, KIND, false>(r, t, one, s.sum, s.sum1); });
             s.sum = wave_sum(s.sum);
@@ -509,9 +519,9 @@ __global__ __launch_bounds__(THREADS, WAVES) void distill_kernel(Distill a)
         return smooth<KIND>(exp2_fast(t.of_value(v)), KIND == kTwo ? exp2_fast(one.of_value(v)) : 0.0f, f);
     };
     if (grad) {
-        if (!true || t.one_step())
+        if (!kOneStep || t.one_step())
             runs([&](uint32_t at, u32x4 r) {
-                const u32x4 g = run_grad<T, KIND, true>(r, t, one, f);
+                const u32x4 g = run_grad<T, KIND, kOneStep>(r, t, one, f);
                 if (at < cut.end)
                     store_run_once<T>(grad + at, g);
             });
