@@ -374,7 +374,7 @@ __global__ __launch_bounds__(THREADS, WAVES) void distill_kernel(Distill a)
         if (has_entry)
             id = entry.id(c);
         wrong |= id >= c.vocab;
-        if (id >= c.vocab)
+        if (id < 0 || id >= c.vocab)  // and so 32 bits hold it
             id = -1;
         entry.x = load_bits<T>(x + (id >= 0 ? id : 0));
     }

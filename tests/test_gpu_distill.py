@@ -149,6 +149,16 @@ def test_ids_that_occur_several_times():
             assert torch.equal(got[0][1], got[1][1]) and torch.equal(got[0][0], got[1][0])
 
 
+def test_any_negative_id_is_an_empty_entry():
+    """Also one whose low 32 bits are the id of an entry behind it, or the label."""
+    for dtype in TYPES:
+        x, t, ids, y = _inputs(4, 203, 6, dtype, seed=51, ignored=0.0)
+        ids[0], y[0] = torch.tensor([-(1 << 32), 0, 9, -1, 4, 2]), 1
+        ids[1], y[1] = torch.tensor([-(1 << 32) + 5, -(1 << 40) + 7, 1, 2, 5, 3]), 7
+        ids[2] = -(1 << 63)
+        _check(x, t, ids, y, temperature=2.0, label_weight=0.5)
+
+
 def test_what_is_wrong_makes_its_row_nan_and_no_other():
     x, t, ids, y = _inputs(7, 203, 5, torch.bfloat16, seed=11, ignored=0.0)
     good = (x.clone(), t.clone(), ids.clone(), y.clone())
