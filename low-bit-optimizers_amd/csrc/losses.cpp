@@ -6,11 +6,13 @@
 // logits took 120 us of host time for 25 us of kernels (forward 26, of it checks and records 10; the engine itself 30).
 //
 // Errors are Python's: RuntimeError for tensors that do not fit, ValueError for values.  What needs no GPU is checked first.
+#include <ATen/SavedTensorHooks.h>
 #include <ATen/core/Tensor.h>
 #include <ATen/ops/empty.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/core/GradMode.h>
 #include <c10/hip/HIPStream.h>
+#include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/functions/utils.h>
@@ -173,7 +175,39 @@ Tensor once(Tensor grad, const torch::autograd::Edge &input, const char *name)
     return grad;
 }
 
-SavedVariable kept(const Tensor &t) { return t.defined() ? SavedVariable(t, false) : SavedVariable(); }
+// What a backward pass reads again.  Hooks on saved tensors (checkpointing, offloading) may give back another tensor of the same values, so its
+// address is taken where it comes back; what does not fit the call's records is refused.
+struct Kept {
+    SavedVariable variable;
+    std::vector<int64_t> shape;
+    at::ScalarType type = at::kFloat;
+    bool some = false;
+
+    void keep(const Tensor &t)
+    {
+        if (!t.defined())
+            return;
+        some = true;
+        shape = t.sizes().vec();
+        type = t.scalar_type();
+        variable = SavedVariable(t, false);
+    }
+    // also checks that nothing was written over since the loss was computed
+    Tensor back(c10::Device device) const
+    {
+        const Tensor t = variable.unpack();
+        REQUIRE(!some || (t.defined() && t.device() == device && t.scalar_type() == type && t.sizes() == shape), "a saved tensor of ", type, ", shape ",
+                at::IntArrayRef(shape), " on ", device, " came back from its hooks as another");
+        return t;
+    }
+    Tensor back_contiguous(c10::Device device) const
+    {
+        const Tensor t = back(device);
+        return t.defined() ? t.contiguous() : t;
+    }
+};
+
+bool saved_tensors_have_hooks() { return at::SavedTensorDefaultHooks::get_hooks().has_value(); }
 
 // ---------------------------------------------------------------------------------------
 // distillation
@@ -181,13 +215,14 @@ SavedVariable kept(const Tensor &t) { return t.defined() ? SavedVariable(t, fals
 
 // The gradient of a reduced loss is written by the pass that computes the loss, while the row's logits are at hand, for the gradient 1
 // that loss.backward() starts from; a backward pass that arrives with another value writes it again from the logits.
-// float16 training scales its loss as a rule, so there, and for the losses of single rows, only the backward pass writes it.
+// float16 training scales its loss as a rule, so there, and for the losses of single rows, only the backward pass writes it; nor is it made
+// where hooks keep saved tensors elsewhere, to have the memory.
 struct DistillLossBackward : public Node {
-    lpmm_distill_call call;  // its addresses are those of the tensors below, which `apply` unpacks before it uses them
+    lpmm_distill_call call;  // its addresses are set by `apply`
     c10::Device device = c10::kCPU;
     std::vector<int64_t> shape;
     at::TensorOptions options;
-    SavedVariable rows, teacher, ids, labels, scale, map, work;
+    Kept rows, teacher, ids, labels, scale, map, work;
     Tensor grad;  // made along with the loss
 
     variable_list apply(variable_list &&grads) override
@@ -196,10 +231,15 @@ struct DistillLossBackward : public Node {
         Tensor grad_loss = grads[0];
         if (!grad_loss.defined())
             return {Tensor()};
-        // also checks that nothing was written over since the loss was computed
-        const Tensor held[] = {rows.unpack(), teacher.unpack(), ids.unpack(), labels.unpack(), scale.unpack(), map.unpack(), work.unpack()};
-        (void)held;
         const c10::DeviceGuard guard(device);
+        Tensor x = rows.back(device);
+        std::optional<Rows> strides = row_strides(x);
+        if (!strides) {
+            x = x.contiguous();
+            strides = row_strides(x);
+        }
+        const Tensor held[] = {teacher.back_contiguous(device), ids.back_contiguous(device), labels.back_contiguous(device),
+                               scale.back_contiguous(device), map.back_contiguous(device), work.back_contiguous(device)};
         Tensor out = std::move(grad);  // handed out once: a second pass over the graph gets a gradient of its own
         grad.reset();
         const bool made = out.defined();
@@ -215,6 +255,18 @@ struct DistillLossBackward : public Node {
             }
         }
         lpmm_distill_call c = call;
+        c.logits = x.data_ptr();
+        c.inner = strides->inner;
+        c.outer_stride = strides->outer_stride;
+        c.inner_stride = strides->inner_stride;
+        c.teacher = data<void>(held[0]);
+        c.ids = data<void>(held[1]);
+        c.labels = data<int64_t>(held[2]);
+        c.teacher_scale = data<float>(held[3]);
+        c.teacher_map = data<float>(held[4]);
+        c.row_stats = data<float>(held[5]);
+        c.share = c.row_stats + 4 * c.rows;
+        c.row_loss = c.loss = nullptr;
         c.grad = out.data_ptr();
         check(lpmm_distill_loss_grad(&c, static_cast<const float *>(grad_loss.data_ptr()), stride, made, stream_of(device)), "distill_loss_grad");
         return {once(std::move(out), next_edge(0), "distill_loss")};
@@ -223,8 +275,8 @@ struct DistillLossBackward : public Node {
     void release_variables() override
     {
         std::lock_guard<std::mutex> lock(mutex_);
-        for (SavedVariable *v : {&rows, &teacher, &ids, &labels, &scale, &map, &work})
-            v->reset_data();
+        for (Kept *v : {&rows, &teacher, &ids, &labels, &scale, &map, &work})
+            v->variable.reset_data();
         grad.reset();
     }
 
@@ -309,7 +361,7 @@ Tensor distill_loss(const Tensor &logits, const Tensor &teacher_logits, const Te
     c.row_loss = none ? data<float>(loss) : at + stats + 1;
     c.loss = none ? nullptr : data<float>(loss);
     Tensor grad;
-    if (wants_grad && !none && c.type != LPMM_TYPE_F16)
+    if (wants_grad && !none && c.type != LPMM_TYPE_F16 && !saved_tensors_have_hooks())
         grad = at::empty(logits.sizes(), logits.options());
     c.grad = data<void>(grad);
     check(lpmm_distill_loss(&c, stream_of(device)), "distill_loss");
@@ -322,13 +374,13 @@ Tensor distill_loss(const Tensor &logits, const Tensor &teacher_logits, const Te
     node->device = device;
     node->shape = logits.sizes().vec();
     node->options = logits.options();
-    node->rows = kept(rows);
-    node->teacher = kept(teacher);
-    node->ids = kept(ids);
-    node->labels = kept(y);
-    node->scale = kept(or_none(scale));
-    node->map = kept(or_none(qmap));
-    node->work = kept(work);
+    node->rows.keep(rows);
+    node->teacher.keep(teacher);
+    node->ids.keep(ids);
+    node->labels.keep(y);
+    node->scale.keep(or_none(scale));
+    node->map.keep(or_none(qmap));
+    node->work.keep(work);
     node->grad = std::move(grad);
     torch::autograd::set_history(loss, node);
     return loss;
@@ -338,22 +390,32 @@ Tensor distill_loss(const Tensor &logits, const Tensor &teacher_logits, const Te
 // balance of experts
 // ---------------------------------------------------------------------------------------
 struct BalanceLossBackward : public Node {
-    lpmm_balance_call call;
+    lpmm_balance_call call;  // its addresses are set by `apply`
     c10::Device device = c10::kCPU;
     std::vector<int64_t> shape;
     at::TensorOptions options;
-    SavedVariable rows, mask, factors;
+    Kept rows, mask, factors;
 
     variable_list apply(variable_list &&grads) override
     {
         std::lock_guard<std::mutex> lock(mutex_);
         if (!grads[0].defined())
             return {Tensor()};
-        const Tensor held[] = {rows.unpack(), mask.unpack(), factors.unpack()};
-        (void)held;
         const c10::DeviceGuard guard(device);
+        Tensor x = rows.back(device);
+        if (x.stride(-1) != 1)
+            x = x.contiguous();
+        const Tensor seen = mask.back_contiguous(device), f = factors.back_contiguous(device);
         Tensor out = at::empty(shape, options);
         lpmm_balance_call c = call;
+        c.logits = x.data_ptr();
+        c.outer_stride = x.dim() == 3 ? x.stride(0) : 0;
+        c.inner_stride = x.stride(-2);
+        c.mask = data<uint8_t>(seen);
+        c.factors = data<float>(f);
+        c.ids = c.work = nullptr;
+        c.counts = nullptr;
+        c.loss = nullptr;
         c.grad = out.data_ptr();
         check(lpmm_balance_loss_grad(&c, static_cast<const float *>(grads[0].data_ptr()), stream_of(device)), "balance_loss_grad");
         return {once(std::move(out), next_edge(0), "balance_loss")};
@@ -362,8 +424,8 @@ struct BalanceLossBackward : public Node {
     void release_variables() override
     {
         std::lock_guard<std::mutex> lock(mutex_);
-        for (SavedVariable *v : {&rows, &mask, &factors})
-            v->reset_data();
+        for (Kept *v : {&rows, &mask, &factors})
+            v->variable.reset_data();
     }
 
     std::string name() const override { return "BalanceLossBackward"; }
@@ -419,9 +481,9 @@ std::pair<Tensor, Tensor> balance_loss(const Tensor &router_logits, const Tensor
         node->device = device;
         node->shape = router_logits.sizes().vec();
         node->options = router_logits.options();
-        node->rows = kept(rows);
-        node->mask = kept(seen);
-        node->factors = kept(factors);
+        node->rows.keep(rows);
+        node->mask.keep(seen);
+        node->factors.keep(factors);
         torch::autograd::set_history(loss, node);
     }
     return {loss, counts};
@@ -431,8 +493,9 @@ std::pair<Tensor, Tensor> balance_loss(const Tensor &router_logits, const Tensor
 
 PYBIND11_MODULE(_losses, m)
 {
-    m.def("distill_loss", &distill_loss);
-    m.def("balance_loss", &balance_loss);
+    // wrapped: an exception raised by a hook on a saved tensor stays the Python exception that it is
+    m.def("distill_loss", torch::wrap_pybind_function(&distill_loss));
+    m.def("balance_loss", torch::wrap_pybind_function(&balance_loss));
     m.def("row_strides", [](const Tensor &t) -> std::optional<std::tuple<int64_t, int64_t, int64_t>> {
         const std::optional<Rows> r = row_strides(t);
         if (!r)

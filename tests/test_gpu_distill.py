@@ -472,3 +472,63 @@ def test_a_training_step_with_a_stored_teacher():
         before = head.detach().clone()
         opt.step()
         assert not torch.equal(before, head)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_saved_tensors_that_come_back_elsewhere(dtype):
+    """Hooks that keep saved tensors on the host, with other strides when they come back; what was on the device is overwritten by then."""
+    x, t, ids, y = _inputs(6, 517, 6, dtype, seed=52)
+    whole = torch.randn(6, 600, device="cuda").to(dtype)
+    whole[:, 30:547] = x.cuda()
+    args = [_cuda(a) for a in (t, ids, y)]
+    view, router = whole.detach()[:, 30:547].requires_grad_(True), whole.detach()[:, 30:47].requires_grad_(True)
+    picks = torch.randint(0, 17, (6, 2))
+    mask = torch.tensor([True, False, True, True, True, False], device="cuda")
+    with torch.autograd.graph.saved_tensors_hooks(lambda v: v.cpu(), lambda v: v.cuda().contiguous()):
+        loss = F.distill_loss(view, args[0], args[1], labels=args[2], temperature=2.0, label_weight=0.5)
+        aux, _ = F.balance_loss(router, picks.cuda(), mask=mask, weight=0.5, z_weight=0.1)
+    for a in (whole, *args, mask):
+        a.zero_()
+    grads = torch.autograd.grad(loss, view)[0], torch.autograd.grad(aux, router)[0]
+    want, bound, grad, gbound = ref.distill(x, t, ids, 2.0, y, 1.0, 0.5)
+    ref.assert_within(loss, want, bound, "loss")
+    ref.assert_within(grads[0], grad, gbound, "gradient")
+    want, bound, _, grad, gbound = ref.balance(x[:, :17], picks, torch.tensor([True, False, True, True, True, False]), 0.5, 0.1)
+    ref.assert_within(aux, want, bound, "balance")
+    ref.assert_within(grads[1], grad, gbound, "gradient of the balance")
+
+
+def test_saved_tensors_that_come_back_as_others_are_refused():
+    x, t, ids, y = _inputs(6, 517, 6, torch.float32, seed=53)
+    for unpack in (lambda v: v, lambda v: v.cuda()[:1], lambda v: v.cuda().double()):
+        leaf = x.cuda().requires_grad_(True)
+        with torch.autograd.graph.saved_tensors_hooks(lambda v: v.cpu(), unpack):
+            loss = F.distill_loss(leaf, t.cuda(), ids.cuda())
+            aux, _ = F.balance_loss(leaf, ids.cuda())
+        for out in (loss, aux):
+            with pytest.raises(RuntimeError, match="came back from its hooks"):
+                out.backward()
+
+
+@pytest.mark.parametrize("reentrant", [False, True])
+def test_inside_a_checkpoint(reentrant):
+    """The head and its loss by chunks of rows, made again in the backward pass; no logits are kept between."""
+    from torch.utils.checkpoint import checkpoint
+
+    rows, vocab, width = 64, 5003, 16
+    g = torch.Generator().manual_seed(54)
+    h = torch.randn(rows, width, generator=g).cuda().requires_grad_(True)
+    head = (torch.randn(vocab, width, generator=g) * 0.3).cuda().requires_grad_(True)
+    _, t, ids, y = (_cuda(a) for a in _inputs(rows, vocab, 8, torch.float32, seed=55))
+
+    def part(h, cut):
+        return F.distill_loss(h @ head.t(), t[cut], ids[cut], labels=y[cut], label_weight=0.5, temperature=2.0, reduction="sum")
+
+    whole = torch.autograd.grad(sum(part(h[n:n + 16], slice(n, n + 16)) for n in range(0, rows, 16)), (h, head))
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    loss = sum(checkpoint(part, h[n:n + 16], slice(n, n + 16), use_reentrant=reentrant) for n in range(0, rows, 16))
+    assert torch.cuda.memory_allocated() - before < 16 * vocab * 4
+    loss.backward()
+    for got, want in zip((h.grad, head.grad), whole):
+        assert torch.allclose(got, want, rtol=1e-4, atol=1e-4 * float(want.abs().max()))
