@@ -887,12 +887,15 @@ typedef struct lpmm_balance_call {
     float *factors;             /* [groups][experts + 2]: what the gradient call needs */
     void *work;                 /* lpmm_balance_work_bytes, 8-byte aligned; free again when the call's kernels have run */
     void *grad;                 /* gradient call only: [groups][tokens][experts] of `type` */
-    int64_t groups, tokens, experts, picks; /* experts: 1 .. LPMM_BALANCE_MOST; picks: 0 .. experts; groups * tokens and tokens * picks below 2^31 */
+    int64_t groups, tokens, experts, picks; /* experts: 1 .. LPMM_BALANCE_MOST; picks: 0 .. experts; groups: 0 .. LPMM_BALANCE_GROUPS; groups * tokens at
+                                               most LPMM_BALANCE_TOKENS, tokens * picks below 2^31 */
     int64_t outer_stride, inner_stride;
     float weight, z_weight;
     int32_t type, id_bits;
 } lpmm_balance_call;
 #define LPMM_BALANCE_MOST 1024
+#define LPMM_BALANCE_GROUPS 65535
+#define LPMM_BALANCE_TOKENS (1 << 28)
 
 int64_t lpmm_balance_work_bytes(int64_t groups, int64_t tokens, int64_t experts);
 int lpmm_balance_loss(const lpmm_balance_call *call, void *stream);

@@ -388,8 +388,10 @@ int check_call(const lpmm_balance_call &c)
 {
     if (c.type < LPMM_TYPE_F32 || c.type > LPMM_TYPE_BF16 || (c.id_bits != 32 && c.id_bits != 64) || !isfinite(c.weight) || !isfinite(c.z_weight))
         return LPMM_ERR_ARG;
-    if (c.experts < 1 || c.experts > LPMM_BALANCE_MOST || c.picks < 0 || c.picks > c.experts || c.groups < 0 || c.groups > (int64_t)1 << 24 ||
-        c.tokens < 0 || c.tokens > INT32_MAX || c.tokens * (c.picks > 0 ? c.picks : 1) > INT32_MAX || c.groups * c.tokens > INT32_MAX || c.outer_stride < 0 || c.inner_stride < 0)
+    // groups and tokens: a launch's threads are counted in 32 bits, 1024 to 16 experts of a group, 256 to 32 tokens
+    if (c.experts < 1 || c.experts > LPMM_BALANCE_MOST || c.picks < 0 || c.picks > c.experts || c.groups < 0 || c.groups > LPMM_BALANCE_GROUPS ||
+        c.tokens < 0 || c.tokens > LPMM_BALANCE_TOKENS || c.tokens * (c.picks > 0 ? c.picks : 1) > INT32_MAX ||
+        c.groups * c.tokens > LPMM_BALANCE_TOKENS || c.outer_stride < 0 || c.inner_stride < 0)
         return LPMM_ERR_SIZE;
     LPMM_REQUIRE_ALIGN(c.factors, 4);
     if (c.groups == 0)

@@ -30,11 +30,13 @@ enum Shared {
     kCountHere,  // few rows: every workgroup counts them, a microsecond each at once, for a launch less
 };
 constexpr int64_t kFewRows = 256;  // at most a workgroup's threads
+constexpr int64_t kMostRows = (int64_t)1 << 21;  // of a launch, whose threads are counted in 32 bits
 
 struct Distill {
     lpmm_distill_call c;
     const float *grad_loss;  // the gradient call: not NULL
     int64_t grad_loss_stride;
+    int64_t first;    // row of the launch's first workgroup
     int made;         // the gradient call: grad holds what belongs to grad_loss == 1
     int shared;       // enum Shared
     int with_label;   // labels that have a weight
@@ -304,7 +306,7 @@ __global__ __launch_bounds__(THREADS, WAVES) void distill_kernel(Distill a)
     __shared__ OfWave room[kWaves];
     extern __shared__ __attribute__((aligned(16))) int entries[];
     const lpmm_distill_call &c = a.c;
-    const int64_t row = blockIdx.x;
+    const int64_t row = a.first + blockIdx.x;
     float scale = a.each;
     if constexpr (AGAIN) {
         const float g = a.grad_loss[row * a.grad_loss_stride];
@@ -635,13 +637,16 @@ Distill arguments(const lpmm_distill_call &c)
 }
 
 template <typename T, int KIND, int THREADS, int RUNS, int WAVES>
-void launch(const Distill &a, hipStream_t stream)
+void launch(Distill a, hipStream_t stream)
 {
     const int places = ((int)a.c.topk + 1 + 3) & ~3;
-    if (a.grad_loss)
-        distill_kernel<T, KIND, true, THREADS, RUNS, WAVES><<<(unsigned)a.c.rows, THREADS, places * 8, stream>>>(a);
-    else
-        distill_kernel<T, KIND, false, THREADS, RUNS, WAVES><<<(unsigned)a.c.rows, THREADS, places * 8, stream>>>(a);
+    for (; a.first < a.c.rows; a.first += kMostRows) {
+        const unsigned rows = (unsigned)(a.c.rows - a.first < kMostRows ? a.c.rows - a.first : kMostRows);
+        if (a.grad_loss)
+            distill_kernel<T, KIND, true, THREADS, RUNS, WAVES><<<rows, THREADS, places * 8, stream>>>(a);
+        else
+            distill_kernel<T, KIND, false, THREADS, RUNS, WAVES><<<rows, THREADS, places * 8, stream>>>(a);
+    }
 }
 
 template <typename T, int KIND>

@@ -227,3 +227,23 @@ def test_nothing_is_written_past_the_tokens():
     _, _, wcounts, wgrad, gbound = ref.balance(r.cpu(), ids.cpu(), mask.cpu(), 0.5, 0.1)
     assert torch.equal(room[1][pad:-pad].view(3, 13).cpu(), wcounts)
     ref.assert_within(room[4][pad:-pad].view(3, 67, 13), wgrad, gbound, "gradient")
+
+
+@pytest.mark.parametrize("shape,experts", [((65535, 1), 5), ((65535, 2), 1024), ((1 << 22,), 2)])
+def test_the_most_groups_and_many_tokens(shape, experts):
+    """Each group by itself is what a call on some of them gives, up to the division by their number."""
+    r = torch.randn(*shape, experts, device="cuda").to(torch.bfloat16).requires_grad_(True)
+    ids = torch.randint(0, experts, (*shape, 1), device="cuda")
+    loss, counts = F.balance_loss(r, ids, weight=0.5, z_weight=0.1)
+    grad = torch.autograd.grad(loss, r)[0]
+    assert int(counts.sum()) == ids.numel() and loss.isfinite() and not grad.isnan().any()
+    if len(shape) == 2:
+        some = slice(shape[0] - 8, shape[0])
+        want, bound, wcounts, wgrad, gbound = ref.balance(r.detach()[some].cpu(), ids[some].cpu(), None, 0.5, 0.1, 8.0 / shape[0])
+        assert torch.equal(counts[some].cpu(), wcounts)
+        ref.assert_within(grad[some], wgrad, gbound, "gradient")
+    else:
+        want, bound, wcounts, wgrad, gbound = ref.balance(r.detach().cpu(), ids.cpu(), None, 0.5, 0.1)
+        assert torch.equal(counts.cpu(), wcounts)
+        ref.assert_within(loss, want, bound, "loss")
+        ref.assert_within(grad, wgrad, gbound, "gradient")

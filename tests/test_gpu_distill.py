@@ -438,6 +438,23 @@ def test_offsets_past_32_bits():
     assert loss.isfinite()
 
 
+def test_more_rows_than_a_launch_has():
+    """Short rows, so many that their threads do not fit 32 bits: the last rows are what a call on them alone gives."""
+    rows, vocab = (1 << 24) + 5, 3
+    x = torch.randn(rows, vocab, device="cuda").requires_grad_(True)
+    t, ids = torch.randn(rows, 2, device="cuda"), torch.randint(-1, vocab, (rows, 2), device="cuda", dtype=torch.int32)
+    weight = torch.rand(rows, device="cuda")
+    loss = F.distill_loss(x, t, ids, temperature=2.0, reduction="none")
+    grad = torch.autograd.grad(loss, x, weight)[0]
+    whole = F.distill_loss(x.detach(), t, ids, temperature=2.0, reduction="sum")
+    for cut in (slice(rows - 7, rows), slice((1 << 21) - 2, (1 << 21) + 2)):
+        part = x.detach()[cut].clone().requires_grad_(True)
+        alone = F.distill_loss(part, t[cut], ids[cut], temperature=2.0, reduction="none")
+        assert torch.equal(alone, loss[cut]) and torch.equal(torch.autograd.grad(alone, part, weight[cut])[0], grad[cut])
+    total = float(loss.detach().double().sum())  # the sum is in 64 bits, and rounded once
+    assert abs(float(whole) - total) <= 2 * ref.U * abs(total)
+
+
 def test_a_training_step_with_a_stored_teacher():
     """As it is used: the teacher's top logits stored in 8 bits, the student's loss with the balance of its router, 4-bit optimizer steps."""
     torch.manual_seed(50)

@@ -87,6 +87,9 @@ def test_stored_teacher_refuses(error, text, change, codes):
     (RuntimeError, "experts are supported", dict(router_logits=torch.randn(5, 1025))),
     (RuntimeError, "experts are supported", dict(router_logits=torch.randn(5, 0))),
     (RuntimeError, "3 picks of 2", dict(router_logits=torch.randn(5, 2), expert_ids=torch.zeros(5, 3, dtype=torch.int64))),
+    (RuntimeError, "at most 65535 groups", dict(router_logits=torch.zeros(1, 1, 1).expand(65536, 1, 1), expert_ids=torch.zeros(65536, 1, 1, dtype=torch.int32))),
+    (RuntimeError, "tokens in all", dict(router_logits=torch.zeros(1, 1, 1).expand(2, 2 ** 27 + 1, 1),
+                                         expert_ids=torch.zeros(1, 1, 0, dtype=torch.int32).expand(2, 2 ** 27 + 1, 0))),
     (RuntimeError, "mask must be a bool tensor", dict(mask=torch.ones(5))),
     (RuntimeError, "mask must be a bool tensor", dict(mask=torch.ones(5, 1, dtype=torch.bool))),
     (ValueError, "weight must be finite", dict(weight=math.nan)),
@@ -175,6 +178,8 @@ def _balance_record(**change):
     (ALIGN, dict(loss=2), False), (ALIGN, dict(grad=2), True), (ALIGN, dict(factors=2), True),
     (SIZE, dict(experts=0), False), (SIZE, dict(experts=1025), False), (SIZE, dict(picks=9), False), (SIZE, dict(picks=-1), False),
     (SIZE, dict(groups=-1), False), (SIZE, dict(tokens=-1), False), (SIZE, dict(tokens=2 ** 30), False), (SIZE, dict(inner=-8), True),
+    (SIZE, dict(groups=65536), False), (SIZE, dict(groups=65536, tokens=0), True), (SIZE, dict(tokens=2 ** 28 + 1), True),
+    (SIZE, dict(groups=3, tokens=2 ** 27), False),
     (ARG, dict(type=3), False), (ARG, dict(id_bits=8), False), (ARG, dict(weight=math.nan), False), (ARG, dict(z_weight=math.inf), True),
     (0, dict(groups=0), True), (0, dict(tokens=0), True),
 ])
