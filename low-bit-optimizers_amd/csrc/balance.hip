@@ -10,6 +10,12 @@
 // within a row of lanes (no shared memory) and every load of a wave covers whole stretches of several tokens.  A thread keeps the sums of
 // its experts' probabilities over all the tokens that pass through it; lanes, waves and workgroups are joined in a fixed order.  Counts are
 // integers: the order of their atomics, in shared memory only, does not change them.
+//
+// 65536 x 256 fp32, 8 picks, masked (67 MB of logits): sums 18 us, join 12, gradient 22 (134 MB, 6.2 TB/s).  Where a lane had 16
+// values side by side, so that the lanes of a load lay 64 bytes apart, and each turn waited for its own loads, sums and gradient took 92 and 120.  The join is
+// a chain of reads of what 512 workgroups left, one workgroup to 16 experts; with one to all experts of a group it took 71.  At 16 x 8 a
+// single workgroup does sums and join in 7 us.  Up to some 16384 x 64 the calls are bound by the host (54-64 us of loss and gradient, of them
+// torch's own engine 42).
 #include "losses.hpp"
 
 namespace lpmm {

@@ -11,8 +11,8 @@
 // long to hold are read twice.
 //
 // Bound by memory: without any exponential the kernel takes as long (8188 x 32000 bf16: 203 us with them, 206 without).  Loss and gradient of that
-// batch, a tenth of its rows left out by their labels, move 1.00 GB in 188 us, 5.3 TB/s, where a copy of 4 GB by the library reaches 4.9; evaluation
-// alone reads 6.2 TB/s.  What a row costs beside its bytes is a chain of some 7 us (label, entries, logits at the entries, two barriers,
+// batch, a tenth of its rows left out by their labels, move 1.00 GB in 181-188 us, 5.3-5.5 TB/s, where a copy of 4 GB by the library reaches 4.9;
+// evaluation alone reads 6.0 TB/s.  What a row costs beside its bytes is a chain of some 7 us (label, entries, logits at the entries, two barriers,
 // the last stores), hidden by the other workgroups of a compute unit; rows over 65536 16-bit values leave room for one, and move 4.7 TB/s.
 //
 // The gradient belongs to the loss's own pass because the row is at hand there: 4 bytes a bf16 value where a second pass moves 6.

@@ -13,6 +13,8 @@ Where the reference chains abs / max / div / cat / pack (and unpack / mul) as se
 passes, each call here is one HIP kernel (two for rank-1 quantisation: statistics, then
 normalise + search + pack; tensors of 3..8 dimensions add a kernel that folds the leading
 dimensions' statistics into one scale per row of the (numel / last, last) view).
+
+`distill_loss` and `balance_loss` (lpmm/losses.py) are terms of a training loss with their gradients.
 """
 import ctypes
 import math
