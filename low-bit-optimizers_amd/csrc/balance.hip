@@ -11,10 +11,10 @@
 // its experts' probabilities over all the tokens that pass through it; lanes, waves and workgroups are joined in a fixed order.  Counts are
 // integers: the order of their atomics, in shared memory only, does not change them.
 //
-// 65536 x 256 fp32, 8 picks, masked (67 MB of logits): sums 18 us, join 12, gradient 22 (134 MB, 6.2 TB/s).  Where a lane had 16
+// 65536 x 256 fp32, 8 picks, masked (67 MB of logits): sums 18 us, join 9, gradient 22 (134 MB, 6.2 TB/s).  Where a lane had 16
 // values side by side, so that the lanes of a load lay 64 bytes apart, and each turn waited for its own loads, sums and gradient took 92 and 120.  The join is
-// a chain of reads of what 512 workgroups left, one workgroup to 16 experts; with one to all experts of a group it took 71.  At 16 x 8 a
-// single workgroup does sums and join in 7 us.  Up to some 16384 x 64 the calls are bound by the host (54-64 us of loss and gradient, of them
+// a chain of reads of what 512 workgroups left, one workgroup to 16 experts and one barrier before its results; with one to all experts of a group it
+// took 71.  At 16 x 8 a single workgroup does sums and join in 6 us.  Up to some 16384 x 64 the calls are bound by the host (54-64 us of loss and gradient, of them
 // torch's own engine 42).
 #include "losses.hpp"
 
@@ -22,7 +22,7 @@ namespace lpmm {
 namespace {
 
 constexpr int kBalThreads = 256, kBalWaves = kBalThreads / kWave, kLanes = 16;
-constexpr int kJoinThreads = 1024, kJoinColumns = 16, kJoinSlices = kJoinThreads / kJoinColumns;
+constexpr int kJoinThreads = 1024, kJoinColumns = 16;
 
 struct Balance {
     lpmm_balance_call c;
@@ -143,24 +143,31 @@ __device__ __forceinline__ float softmax(const u32x4 (&raw)[CHUNKS], int lanes, 
     return m + logf(s);
 }
 
-// Joins the parts of kJoinColumns experts of a group: counts, the gradient's factors, this tile's part of the loss.  The tile that comes
-// last adds up the parts of the loss, in their order.
+// What the waves of a workgroup hand to its first one.
 template <int THREADS>
-__device__ __forceinline__ void join(const Balance &a, int64_t group, int tile, double *room, double (*sums)[kJoinColumns])
+struct Joined {
+    static constexpr int kWaves = THREADS / kWave;
+    double prob[kWaves][kJoinColumns], count[kWaves][kJoinColumns], square[kWaves], tokens[kWaves];
+    int wrong[kWaves];
+    bool last;
+};
+
+// Joins the parts of kJoinColumns experts of a group: counts, the gradient's factors, this tile's part of the loss.  The tile that comes
+// last adds up the parts of the loss, in their order.  Sixteen lanes that lie side by side take a part's experts, a wave four parts at a time.
+template <int THREADS>
+__device__ __forceinline__ void join(const Balance &a, int64_t group, int tile, Joined<THREADS> &room)
 {
     const lpmm_balance_call &c = a.c;
-    constexpr int kSlices = THREADS / kJoinColumns;
-    const int tid = threadIdx.x, experts = (int)c.experts, column = tid % kJoinColumns, slice = tid / kJoinColumns, e = tile * kJoinColumns + column;
+    constexpr int kSlices = THREADS / kJoinColumns, kWaves = THREADS / kWave;
+    const int tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave, experts = (int)c.experts;
+    const int column = tid % kJoinColumns, slice = tid / kJoinColumns, e = tile * kJoinColumns + column;
     const int64_t base = group * a.parts;
-    double square = 0.0, tokens = 0.0;
-    bool wrong = false;
-    for (int64_t p = tid; p < a.parts; p += THREADS) {
-        square += a.square[base + p];
-        const int seen = a.seen[base + p];
-        wrong |= seen < 0;
-        tokens += (double)(seen < 0 ? -1 - seen : seen);
+    double square = 0.0, prob = 0.0;
+    int seen = 0;
+    if (tid < a.parts) {  // at most as many as the workgroup has threads: split
+        square = a.square[base + tid];
+        seen = a.seen[base + tid];
     }
-    double prob = 0.0;
     int64_t picked = 0;
     if (e < experts) {
         for (int64_t p = slice; p < a.parts; p += 8 * kSlices)
@@ -172,66 +179,74 @@ __device__ __forceinline__ void join(const Balance &a, int64_t group, int tile, 
                     picked += a.picked[at];
                 }
     }
-    square = block_sum_f64<THREADS>(square, room);
-    tokens = block_sum_f64<THREADS>(tokens, room);
-    wrong = __syncthreads_or(wrong);
-    sums[slice][column] = prob;
-    __syncthreads();
-    if (slice == 0) {
-        prob = 0.0;
-        for (int i = 0; i < kSlices; ++i)
-            prob += sums[i][column];
+    double count = (double)picked;  // exact
+#pragma unroll
+    for (int o = kJoinColumns; o < kWave; o <<= 1) {
+        prob += __shfl_xor(prob, o, kWave);
+        count += __shfl_xor(count, o, kWave);
     }
+    square = wave_sum_f64(square);
+    double tokens = wave_sum_f64((double)(seen < 0 ? -1 - seen : seen));
+    const bool any_wrong = __any(seen < 0);
+    if (lane < kJoinColumns)
+        room.prob[wave][lane] = prob, room.count[wave][lane] = count;
+    if (lane == 0)
+        room.square[wave] = square, room.tokens[wave] = tokens, room.wrong[wave] = any_wrong;
     __syncthreads();
-    sums[slice][column] = (double)picked;  // exact
-    __syncthreads();
-    double loss = 0.0;
-    const double per = tokens > 0.0 ? 1.0 / tokens : 0.0;
-    if (slice == 0 && e < experts) {
-        double count = 0.0;
-        for (int i = 0; i < kSlices; ++i)
-            count += sums[i][column];
-        const double share = c.picks > 0 ? (double)c.weight * experts * per * per / (double)c.picks : 0.0;
-        c.counts[group * experts + e] = (int64_t)count;
-        c.factors[group * (experts + 2) + e] = wrong ? NAN : (float)(share * count / (double)c.groups);
-        loss = share * count * prob;
-    }
-    loss = block_sum_f64<THREADS>(loss, room);
     const int64_t all = c.groups * a.tiles;
-    __shared__ bool last;
-    if (tid == 0) {
-        if (tile == 0) {
-            c.factors[group * (experts + 2) + experts] = (float)(2.0 * (double)c.z_weight * per / (double)c.groups);
-            c.factors[group * (experts + 2) + experts + 1] = 0.0f;
-            loss = wrong ? NAN : loss + (double)c.z_weight * square * per;
+    if (wave == 0) {
+        prob = count = square = tokens = 0.0;
+        int wrong = 0;
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) {
+            prob += room.prob[w][column];
+            count += room.count[w][column];
+            square += room.square[w];
+            tokens += room.tokens[w];
+            wrong |= room.wrong[w];
         }
-        last = true;
-        if (all == 1) {
-            c.loss[0] = (float)loss;
-            last = false;
-        } else {
-            a.loss_part[group * a.tiles + tile] = loss;
-            __threadfence();
-            last = atomicAdd(a.done, 1u) == (uint32_t)all - 1u;
-            __threadfence();
+        const double per = tokens > 0.0 ? 1.0 / tokens : 0.0;
+        double loss = 0.0;
+        if (lane < kJoinColumns && e < experts) {
+            const double share = c.picks > 0 ? (double)c.weight * experts * per * per / (double)c.picks : 0.0;
+            c.counts[group * experts + e] = (int64_t)count;
+            c.factors[group * (experts + 2) + e] = wrong ? NAN : (float)(share * count / (double)c.groups);
+            loss = share * count * prob;
+        }
+        loss = wave_sum_f64(loss);
+        if (lane == 0) {
+            if (tile == 0) {
+                c.factors[group * (experts + 2) + experts] = (float)(2.0 * (double)c.z_weight * per / (double)c.groups);
+                c.factors[group * (experts + 2) + experts + 1] = 0.0f;
+                loss = wrong ? NAN : loss + (double)c.z_weight * square * per;
+            }
+            bool last = false;
+            if (all == 1) {
+                c.loss[0] = (float)loss;
+            } else {
+                a.loss_part[group * a.tiles + tile] = loss;
+                __threadfence();
+                last = atomicAdd(a.done, 1u) == (uint32_t)all - 1u;
+                __threadfence();
+            }
+            room.last = last;
         }
     }
     __syncthreads();
-    if (!last)
+    if (!room.last)
         return;
     double s = 0.0;
     for (int64_t i = tid; i < all; i += THREADS)
         s += __hip_atomic_load(a.loss_part + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    s = block_sum_f64<THREADS>(s, room);
+    s = block_sum_f64<THREADS>(s, room.square);
     if (tid == 0)
         c.loss[0] = (float)(s / (double)c.groups);
 }
 
 __global__ __launch_bounds__(kJoinThreads) void balance_join_kernel(Balance a)
 {
-    __shared__ double room[kJoinThreads / kWave];
-    __shared__ double sums[kJoinSlices][kJoinColumns];
-    join<kJoinThreads>(a, blockIdx.x / a.tiles, blockIdx.x % a.tiles, room, sums);
+    __shared__ Joined<kJoinThreads> room;
+    join(a, blockIdx.x / a.tiles, blockIdx.x % a.tiles, room);
 }
 
 template <typename T, int CHUNKS>
@@ -318,10 +333,10 @@ __global__ __launch_bounds__(kBalThreads) void balance_sums_kernel(Balance a)
         a.seen[blockIdx.x] = any_wrong ? -1 - all : all;
     }
     if (gridDim.x == 1) {
-        __shared__ double sums[kBalThreads / kJoinColumns][kJoinColumns];
+        __shared__ Joined<kBalThreads> joined;
         __syncthreads();
         for (int tile = 0; tile < a.tiles; ++tile) {
-            join<kBalThreads>(a, 0, tile, room, sums);
+            join(a, 0, tile, joined);
             __syncthreads();
         }
     }
