@@ -266,3 +266,19 @@ def test_definition_of_the_balance():
                 assert abs(want - grad[g, n, e]) < 1e-8
     even = torch.zeros(8, 4)
     assert abs(ref.balance(even, torch.arange(8).view(8, 1) % 4)[0] - 1.0) < 1e-12
+
+
+def test_a_missing_host_side_is_an_error(monkeypatch):
+    import sys
+
+    import lpmm
+    from lpmm import _native
+
+    _native.losses()
+    monkeypatch.setattr(_native, "_losses", None)
+    monkeypatch.delattr(lpmm, "_losses")
+    monkeypatch.setitem(sys.modules, "lpmm._losses", None)
+    with pytest.raises(RuntimeError, match="does not load"):
+        F.distill_loss(**_distill_inputs())
+    with pytest.raises(RuntimeError, match="does not load"):
+        F.balance_loss(torch.randn(5, 8), torch.zeros(5, 2, dtype=torch.int64))
