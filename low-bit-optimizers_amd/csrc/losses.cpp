@@ -132,6 +132,16 @@ void check(int status, const char *what)
 
 void *stream_of(c10::Device device) { return c10::hip::getCurrentHIPStream(device.index()).stream(); }
 
+// Which recording into a graph a stream is in; 0: none.  The default stream is never in one, and is not asked, which is an error during another's.
+unsigned long long recording(void *stream)
+{
+    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+    unsigned long long id = 0;
+    if (!stream || hipStreamGetCaptureInfo(static_cast<hipStream_t>(stream), &status, &id) != hipSuccess || status == hipStreamCaptureStatusNone)
+        return 0;
+    return id;
+}
+
 // Row n of the flattened leading dimensions starts at (n / inner) * outer_stride + (n % inner) * inner_stride.
 struct Rows {
     int64_t inner, outer_stride, inner_stride;
@@ -225,6 +235,7 @@ struct DistillLossBackward : public Node {
     at::TensorOptions options;
     Kept rows, teacher, ids, labels, scale, map, work;
     Tensor grad;  // made along with the loss
+    unsigned long long recorded = 0;  // the recording that made it
 
     variable_list apply(variable_list &&grads) override
     {
@@ -243,6 +254,8 @@ struct DistillLossBackward : public Node {
                                scale.back_contiguous(device), map.back_contiguous(device), work.back_contiguous(device)};
         Tensor out = std::move(grad);  // handed out once: a second pass over the graph gets a gradient of its own
         grad.reset();
+        if (out.defined() && recording(stream_of(device)) != recorded)
+            out.reset();  // every replay has to write it, to memory that is the recording's own
         const bool made = out.defined();
         if (!made)
             out = at::empty(shape, options);
@@ -382,6 +395,7 @@ Tensor distill_loss(const Tensor &logits, const Tensor &teacher_logits, const Te
     node->scale.keep(or_none(scale));
     node->map.keep(or_none(qmap));
     node->work.keep(work);
+    node->recorded = grad.defined() ? recording(stream_of(device)) : 0;
     node->grad = std::move(grad);
     torch::autograd::set_history(loss, node);
     return loss;

@@ -59,7 +59,7 @@ def distill_loss(logits, teacher_logits, teacher_ids, *, temperature=1.0, labels
     label is ignore_index take no part: loss and gradient are 0 whatever they hold, and 'mean' divides by the number of
     the other rows (the mean of no rows is 0).  An id that occurs several times in a row counts with the sum of its
     probabilities.  Nothing is copied to the host to be checked: an id of V or more, a label outside [0, V) that is not
-    ignore_index, and teacher values of NaN or +infinity make the loss and the gradient of their row NaN.
+    ignore_index (whatever its weight), and teacher values of NaN or +infinity make the loss and the gradient of their row NaN.
 
     Returns a float32 tensor: a scalar for reduction 'mean' or 'sum', (...) for 'none'.  No gradient flows to the teacher.  With
     'mean' and 'sum' factors are best put into the two weights: the gradient is then made along with the loss, while a loss

@@ -399,6 +399,30 @@ def test_captured_and_replayed(dtype, scale):
             assert torch.equal(outs[k][0], eager[0]) and torch.equal(outs[k][1], eager[1]), f"turn {turn}, graph {k}"
 
 
+def test_a_recorded_backward_pass_of_an_eager_loss_writes_its_gradient_at_every_replay():
+    stream = torch.cuda.Stream()
+    sets = [_cuda(a) for a in _inputs(20, 3001, 12, torch.bfloat16, seed=56)]
+    torch.cuda.synchronize()
+    with torch.cuda.stream(stream):
+        leaf = sets[0].clone().requires_grad_(True)
+        loss = F.distill_loss(leaf, sets[1], sets[2], labels=sets[3], label_weight=0.5, temperature=2.0)
+        factor = torch.ones((), device="cuda")
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=stream):
+        grad = torch.autograd.grad(loss, leaf, factor, retain_graph=True)[0]
+    torch.cuda.synchronize()
+    want = torch.autograd.grad(loss, leaf)[0]
+    torch.cuda.synchronize()
+    for value in (1.0, 0.5, 1.0):
+        factor.fill_(value)
+        grad.zero_()
+        torch.cuda.synchronize()
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(grad, want * value)  # powers of two
+
+
 def test_nothing_is_written_past_the_rows():
     from lpmm import _native
 
