@@ -234,9 +234,11 @@ __device__ __forceinline__ bool takes_off(const int *ids, const float *part, int
         for (int j = 0; j < k; ++j)
             if (ids[j] == id)
                 return false;
+        double all = off;  // up to 1025 parts, each of which may be as small as what their sum leaves of the smooth term
         for (int j = k + 1; j < entries; ++j)
             if (ids[j] == id)
-                off += part[j];
+                all += part[j];
+        off = (float)all;
     }
     return true;
 }

@@ -573,3 +573,42 @@ def test_inside_a_checkpoint(reentrant):
     loss.backward()
     for got, want in zip((h.grad, head.grad), whole):
         assert torch.allclose(got, want, rtol=1e-4, atol=1e-4 * float(want.abs().max()))
+
+
+def _awkward(x, vocab):
+    """Rows that the sums relative to a thread's first values do not fit: the first half or all but one value masked, a late value far above the rest,
+    values that grow along the row, magnitudes past one step."""
+    x[0, :vocab // 2] = -math.inf
+    x[1, :] = -math.inf
+    x[1, vocab - 3] = 2.0
+    x[2, vocab - 5] = 90.0
+    x[3] = torch.linspace(-60, 60, vocab).to(x.dtype)
+    x[4] = x[4] + 30000.0
+    x[5, ::7] = -math.inf
+    x[6, : vocab // 3] = torch.finfo(x.dtype).min
+    return x
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("vocab,topk", [(100, 300), (4097, 5), (8191, 257), (9000, 600), (16384, 20), (16389, 20), (20001, 513), (32761, 9), (40000, 1024), (60001, 9), (70000, 9), (140001, 9)])
+def test_many_rows_of_every_length(vocab, topk, dtype):
+    """As many rows as the shapes for many rows ask for; what is checked is a part of them, with rows that need their largest value first."""
+    x, t, ids, y = _inputs(10, vocab, topk, dtype, seed=57)
+    x, rows = _awkward(x, vocab), 260
+    t[1], ids[1] = 1.0, vocab - 3  # what the one value left can give
+    ids[0], ids[6] = ids[0].clamp(min=vocab // 2), ids[6].clamp(min=vocab // 2)
+    ids[5] = ids[5].masked_fill(ids[5] % 7 == 0, -1)
+    y[:7] = torch.tensor([vocab - 1, vocab - 3, vocab - 5, vocab - 1, 3, 1, vocab - 2])
+    many = lambda a: a.repeat((rows // 10,) + (1,) * (a.dim() - 1)).cuda()
+    for temperature, wl in ((1.0, 0.5), (2.0, 0.5), (1.5, 0.25)):
+        want, bound, grad, gbound = ref.distill(x, t, ids, temperature, y, 1.0, wl, reduction="none")
+        leaf = many(x).requires_grad_(True)
+        loss = F.distill_loss(leaf, many(t), many(ids), labels=many(y), temperature=temperature, label_weight=wl, reduction="none")
+        loss.backward(torch.ones(rows, device="cuda"))
+        for cut in (slice(0, 10), slice(rows - 10, rows)):
+            ref.assert_within(loss[cut], want, bound, f"T={temperature} loss")
+            ref.assert_within(leaf.grad[cut], grad, gbound, f"T={temperature} gradient")
+        if dtype != torch.float16:  # the gradient that is made along with the loss
+            made = leaf.detach().requires_grad_(True)
+            F.distill_loss(made, many(t), many(ids), labels=many(y), temperature=temperature, label_weight=wl, reduction="sum").backward()
+            ref.assert_within(made.grad[:10], grad, gbound, f"T={temperature} gradient made with the loss")
