@@ -14,8 +14,8 @@
 // 65536 x 256 fp32, 8 picks, masked (67 MB of logits): sums 18 us, join 9, gradient 22 (134 MB, 6.2 TB/s).  Where a lane had 16
 // values side by side, so that the lanes of a load lay 64 bytes apart, and each turn waited for its own loads, sums and gradient took 92 and 120.  The join is
 // a chain of reads of what 512 workgroups left, one workgroup to 16 experts and one barrier before its results; with one to all experts of a group it
-// took 71.  At 16 x 8 a single workgroup does sums and join in 6 us.  Up to some 16384 x 64 the calls are bound by the host (54-64 us of loss and gradient, of them
-// torch's own engine 42).
+// took 71.  At 16 x 8 a single workgroup does sums and join in 6 us.  Up to some 16384 x 64 the calls are bound by the host (54-68 us of loss and gradient, of them
+// torch's own engine 42-47).
 #include "losses.hpp"
 
 namespace lpmm {

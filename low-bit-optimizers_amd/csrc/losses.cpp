@@ -3,8 +3,8 @@
 //
 // In Python the same work bounded every call on less than some ten million logits: a node written in Python takes the interpreter's lock
 // on the engine's thread while the calling thread waits in the engine, and the loss and gradient of 16 rows of 8192
-// logits took 120 us of host time for 25 us of kernels (forward 26, of it checks and records 10; the engine itself 30).  From here it takes 58-63,
-// where torch.autograd.grad of a sum of as many values takes 42.
+// logits took 120 us of host time for 25 us of kernels (forward 26, of it checks and records 10; the engine itself 30).  From here it takes 57-68,
+// where torch.autograd.grad of a sum of as many values takes 42-47.
 //
 // Errors are Python's: RuntimeError for tensors that do not fit, ValueError for values.  What needs no GPU is checked first.
 #include <ATen/SavedTensorHooks.h>
