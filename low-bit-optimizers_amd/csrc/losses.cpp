@@ -320,6 +320,7 @@ Tensor distill_loss(const Tensor &logits, const Tensor &teacher_logits, const Te
     c.id_bits = id_bits(teacher_ids, "teacher_ids");
     c.teacher_group = group;
     c.teacher_bits = (int32_t)bits;
+    REQUIRE(scale.has_value() == qmap.has_value(), "a stored teacher needs both max1 and qmap");
     if (scale) {
         const int64_t entries = teacher_ids.numel(), bytes = bits == 4 ? (entries + 1) / 2 : entries;
         REQUIRE(teacher_logits.scalar_type() == at::kChar && teacher_logits.dim() == 1 && teacher_logits.is_contiguous(),

@@ -36,7 +36,9 @@ def _stored_teacher(quant):
         raise NotImplementedError(f"a stored teacher has codes of 4 to 8 bits, got {bits}")
     if group < 1:
         raise ValueError(f"group size need to be a positive integer, but found {group}")
-    _require_tensors(max1=scale, qmap=qmap)
+    for name, t in (("max1", scale), ("qmap", qmap)):
+        if not isinstance(t, torch.Tensor):  # None too: a stored teacher has both
+            raise TypeError(f"{name} must be a tensor, got {type(t).__name__}")
     return scale, qmap, group, bits
 
 
