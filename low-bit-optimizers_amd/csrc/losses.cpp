@@ -8,10 +8,13 @@
 //
 // Errors are Python's: RuntimeError for tensors that do not fit, ValueError for values.  What needs no GPU is checked first.
 #include <ATen/SavedTensorHooks.h>
+#include <ATen/TracerMode.h>
 #include <ATen/core/Tensor.h>
 #include <ATen/ops/empty.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/core/GradMode.h>
+#include <c10/core/impl/LocalDispatchKeySet.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/function.h>
@@ -88,6 +91,19 @@ bool same_lead(const Tensor &a, const Tensor &b, int64_t but_a, int64_t but_b)
     return a.sizes().slice(0, a.dim() - but_a) == b.sizes().slice(0, b.dim() - but_b);
 }
 
+// The kernels get addresses, and what the graph sees of a call is the node for its backward pass.  Who records operators (torch.jit.trace, make_fx,
+// fake tensors) would record the allocation of the outputs alone and give back memory that nothing wrote, and a forward-mode derivative would
+// come out as zero: both are refused, for the loss and for its backward pass.  Modes that only look on are let through.
+void require_seen(const Tensor &t, const char *name, const char *what)
+{
+    using c10::impl::TorchDispatchModeKey;
+    bool recorded = at::tracer::impl::is_dispatch_enabled() || c10::impl::tls_is_dispatch_key_included(c10::DispatchKey::PreDispatch);
+    for (const TorchDispatchModeKey key : {TorchDispatchModeKey::FAKE, TorchDispatchModeKey::PROXY, TorchDispatchModeKey::FUNCTIONAL})
+        recorded = recorded || c10::impl::TorchDispatchModeTLS::get_mode(key).has_value();
+    REQUIRE(!recorded, what, " cannot be traced: a tracer or fake tensors are active, which do not see its kernels");
+    REQUIRE(!t._fw_grad(0).defined(), name, " has a forward-mode gradient, and ", what, " has no forward-mode derivative");
+}
+
 struct Named {
     const Tensor *tensor;
     const char *name;
@@ -103,6 +119,7 @@ c10::Device device_of(std::initializer_list<Named> tensors)
         if (!device)
             device = t.tensor->device();
         REQUIRE(t.tensor->device() == *device, "all tensors must be on the same device, got ", *device, " and ", t.tensor->device());
+        REQUIRE(t.tensor->numel() == 0 || t.tensor->const_data_ptr(), t.name, " has no memory of its own: a tensor that wraps others is not taken");
     }
     return *device;
 }
@@ -243,6 +260,7 @@ struct DistillLossBackward : public Node {
         Tensor grad_loss = grads[0];
         if (!grad_loss.defined())
             return {Tensor()};
+        require_seen(grad_loss, "the gradient of the loss", "distill_loss");
         const c10::DeviceGuard guard(device);
         Tensor x = rows.back(device);
         std::optional<Rows> strides = row_strides(x);
@@ -301,6 +319,7 @@ Tensor distill_loss(const Tensor &logits, const Tensor &teacher_logits, const Te
                     double teacher_weight, double label_weight, int64_t ignore_index, int reduction, const MaybeTensor &scale,
                     const MaybeTensor &qmap, int64_t group, int64_t bits)
 {
+    require_seen(logits, "logits", "distill_loss");
     lpmm_distill_call c = {};
     REQUIRE_VALUE(temperature >= 1.0 / 1024 && temperature <= 1024.0, "temperature must lie within 1/1024 and 1024, got ", temperature);
     c.temperature = (float)temperature;
@@ -417,6 +436,7 @@ struct BalanceLossBackward : public Node {
         std::lock_guard<std::mutex> lock(mutex_);
         if (!grads[0].defined())
             return {Tensor()};
+        require_seen(grads[0], "the gradient of the loss", "balance_loss");
         const c10::DeviceGuard guard(device);
         Tensor x = rows.back(device);
         if (x.stride(-1) != 1)
@@ -449,6 +469,7 @@ struct BalanceLossBackward : public Node {
 
 std::pair<Tensor, Tensor> balance_loss(const Tensor &router_logits, const Tensor &expert_ids, const MaybeTensor &mask, double weight, double z_weight)
 {
+    require_seen(router_logits, "router_logits", "balance_loss");
     lpmm_balance_call c = {};
     c.weight = finite(weight, "weight");
     c.z_weight = finite(z_weight, "z_weight");

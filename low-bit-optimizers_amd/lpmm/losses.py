@@ -5,7 +5,8 @@ The reference has no counterpart.  The optimizers end a training step; these sta
 teacher's values may come in the block-wise codes in which the optimizers keep their states
 (`lpmm.functional.vectorwise_quant`).  The kernels are in liblpmm_hip.so, their host side in lpmm/_losses.so; there is no
 CPU or PyTorch fallback.  Work is enqueued on torch's current stream of the tensors' device, nothing waits for the GPU,
-and a call can be recorded into a graph.
+and a call can be recorded into a graph.  Inside `torch.compile` a call runs as it is, between two compiled parts.  Tracers
+(`torch.jit.trace`, `make_fx`, fake tensors) and forward-mode derivatives are refused.
 """
 import torch
 

@@ -29,3 +29,64 @@ def test_the_host_side_takes_map_and_scales_together(scale, qmap):
     with pytest.raises(RuntimeError, match="both max1 and qmap"):
         _native.losses().distill_loss(torch.randn(3, 20), torch.zeros(2049, dtype=torch.int8), torch.randint(0, 20, (3, 4)), 1.0, None, 1.0, 0.0,
                                       -100, 2, scale, qmap, 128, 8)
+
+
+def _distill(x):
+    return F.distill_loss(x, torch.zeros(3, 4), torch.arange(12).view(3, 4))
+
+
+def _balance(x):
+    return F.balance_loss(x, torch.zeros(3, 2, dtype=torch.int64))[0]
+
+
+LOSSES = [(_distill, "logits"), (_balance, "router_logits")]
+
+
+@pytest.mark.parametrize("loss,name", LOSSES)
+def test_a_forward_mode_derivative_is_refused(loss, name):
+    """It would come out as zero; the values with which it comes are on the device in earnest, where the same check runs first."""
+    import torch.autograd.forward_ad as forward_ad
+
+    x = torch.randn(3, 20)
+    with forward_ad.dual_level():
+        for dual in (forward_ad.make_dual(x, torch.ones_like(x)), forward_ad.make_dual(torch.randn(6, 20), torch.ones(6, 20))[::2]):
+            with pytest.raises(RuntimeError, match=f"^{name} has a forward-mode gradient"):
+                loss(dual)
+        with pytest.raises(RuntimeError, match="CUDA"):
+            loss(x)
+    with pytest.raises(RuntimeError, match="forward-mode"):
+        torch.func.jvp(loss, (x,), (torch.ones_like(x),))
+
+
+@pytest.mark.parametrize("loss,name", LOSSES)
+def test_tracers_are_refused(loss, name):
+    """They would record the outputs' allocation alone, and give back memory that nothing wrote."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    x = torch.randn(3, 20)
+    with pytest.raises(RuntimeError, match="cannot be traced"):
+        torch.jit.trace(loss, (x,))
+    for kw in (dict(tracing_mode="real"), dict(tracing_mode="fake"), dict(tracing_mode="symbolic"), dict(pre_dispatch=True)):
+        with pytest.raises(RuntimeError, match="cannot be traced"):
+            make_fx(loss, **kw)(x)
+    with FakeTensorMode() as mode, pytest.raises(RuntimeError, match="cannot be traced"):
+        loss(mode.from_tensor(x))
+    with pytest.raises(RuntimeError, match="CUDA"):  # nothing of it stays behind
+        loss(x)
+
+
+class _Wraps(torch.Tensor):
+    @staticmethod
+    def __new__(cls, inner):
+        return torch.Tensor._make_wrapper_subclass(cls, inner.shape, dtype=inner.dtype, device="cuda", strides=inner.stride())
+
+    @classmethod
+    def __torch_dispatch__(cls, func, types, args=(), kwargs=None):
+        raise AssertionError(f"{func} of a wrapper")
+
+
+@pytest.mark.parametrize("loss,name", LOSSES)
+def test_tensors_without_memory_are_refused(loss, name):
+    with pytest.raises(RuntimeError, match=f"{name} has no memory of its own"):
+        loss(_Wraps(torch.randn(3, 20)))
