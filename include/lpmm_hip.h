@@ -21,7 +21,7 @@
 extern "C" {
 #endif
 
-#define LPMM_HIP_ABI_VERSION 2
+#define LPMM_HIP_ABI_VERSION 3 /* grows with every change to a record, and with functions that a binding needs */
 
 /* One quantisation group of the fused path = 128 elements = one scale
  * (lpmm/cpp_extension/fused_adamw_kernel.cu:216-219). */

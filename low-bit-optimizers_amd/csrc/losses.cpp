@@ -541,5 +541,7 @@ PYBIND11_MODULE(_losses, m)
             return std::nullopt;
         return std::make_tuple(r->inner, r->outer_stride, r->inner_stride);
     });
-    m.attr("abi_version") = lpmm_abi_version();
+    // what this module was compiled with: a library of another version would read its records wrongly
+    m.attr("abi_version") = LPMM_HIP_ABI_VERSION;
+    m.attr("record_bytes") = std::make_pair(sizeof(lpmm_distill_call), sizeof(lpmm_balance_call));
 }

@@ -17,7 +17,7 @@ RANK1_MULTI_MAX = 32  # tensors per launch of the two-pass rank-1 step (kR1Max i
 SGD_MULTI_MAX = 64  # tensors per launch of the one-pass SGD step (kSgdMax in csrc/sgd.hip)
 FACTORED_MULTI_MAX = 24  # tensors per launch group of the factored step (kFaMax in csrc/factored.hip)
 V4BIT_MULTI_MAX = 48  # tensors per launch of the one-pass step with an fp32 first moment (kV4Max in csrc/nonfused_m32.hip)
-ABI_VERSION = 2
+ABI_VERSION = 3  # LPMM_HIP_ABI_VERSION
 CODE_TABLE_BYTES = 12288  # LPMM_CODE_TABLE_BYTES
 
 _vp = ctypes.c_void_p
@@ -152,13 +152,13 @@ def lib():
                 f"lpmm: {LIB_PATH} is missing. Build it with `make -C low-bit-optimizers_amd/csrc` "
                 "(hipcc, gfx950). There is no CPU or PyTorch fallback for the quantised optimizer path.")
         handle = ctypes.CDLL(LIB_PATH)
+        version = handle.lpmm_abi_version()  # before anything that another version may not have
+        if version != ABI_VERSION:
+            raise RuntimeError(f"lpmm: liblpmm_hip.so has ABI version {version}, expected {ABI_VERSION}; rebuild it")
         for name, (restype, argtypes) in PROTOTYPES.items():
             fn = getattr(handle, name)
             fn.restype = restype
             fn.argtypes = argtypes
-        if handle.lpmm_abi_version() != ABI_VERSION:
-            raise RuntimeError("lpmm: liblpmm_hip.so has ABI version "
-                               f"{handle.lpmm_abi_version()}, expected {ABI_VERSION}; rebuild it")
         _lib = handle
     return _lib
 
@@ -208,6 +208,8 @@ def losses():
         except ImportError as e:
             raise RuntimeError(f"lpmm: the extension module lpmm/_losses.so does not load ({e}). Build it with "
                                "`make -C low-bit-optimizers_amd/csrc`.") from e
+        if module.abi_version != ABI_VERSION:  # its records would be read wrongly
+            raise RuntimeError(f"lpmm: lpmm/_losses.so was built for ABI version {module.abi_version}, expected {ABI_VERSION}; rebuild it")
         _losses = module
     return _losses
 

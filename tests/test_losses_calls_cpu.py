@@ -90,3 +90,53 @@ class _Wraps(torch.Tensor):
 def test_tensors_without_memory_are_refused(loss, name):
     with pytest.raises(RuntimeError, match=f"{name} has no memory of its own"):
         loss(_Wraps(torch.randn(3, 20)))
+
+
+def _header():
+    import os
+
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    with open(os.path.join(root, "include", "lpmm_hip.h")) as f:
+        return f.read()
+
+
+def test_versions_and_records_are_those_of_the_header():
+    import re
+
+    import losses_ref as ref
+
+    assert int(re.search(r"#define LPMM_HIP_ABI_VERSION (\d+)", _header()).group(1)) == _native.ABI_VERSION
+    assert _native.lib().lpmm_abi_version() == _native.ABI_VERSION
+    assert _native.losses().record_bytes == (ref.DISTILL_CALL.size, ref.BALANCE_CALL.size)
+
+
+def test_a_host_side_of_another_version_is_an_error(monkeypatch):
+    import sys
+    import types
+
+    import lpmm
+
+    _native.losses()
+    stale = types.ModuleType("lpmm._losses")
+    stale.abi_version = _native.ABI_VERSION - 1
+    monkeypatch.setattr(_native, "_losses", None)
+    monkeypatch.setattr(lpmm, "_losses", stale)
+    monkeypatch.setitem(sys.modules, "lpmm._losses", stale)
+    for _ in range(2):
+        with pytest.raises(RuntimeError, match=f"built for ABI version {_native.ABI_VERSION - 1}, expected {_native.ABI_VERSION}; rebuild it"):
+            F.balance_loss(torch.randn(3, 20), torch.zeros(3, 2, dtype=torch.int64))
+
+
+def test_a_library_of_another_version_is_named_before_its_functions_are_looked_up(monkeypatch):
+    class Old:
+        @staticmethod
+        def lpmm_abi_version():
+            return 2
+
+        def __getattr__(self, name):
+            raise AttributeError(f"undefined symbol: {name}")
+
+    monkeypatch.setattr(_native, "_lib", None)
+    monkeypatch.setattr(_native.ctypes, "CDLL", lambda path: Old())
+    with pytest.raises(RuntimeError, match="ABI version 2, expected .*; rebuild it"):
+        _native.lib()
