@@ -487,6 +487,7 @@ std::pair<Tensor, Tensor> balance_loss(const Tensor &router_logits, const Tensor
     REQUIRE(c.picks <= c.experts, c.picks, " picks of ", c.experts, " experts");
     REQUIRE(c.groups <= LPMM_BALANCE_GROUPS && c.tokens <= LPMM_BALANCE_TOKENS && c.groups * c.tokens <= LPMM_BALANCE_TOKENS, "at most ",
             LPMM_BALANCE_GROUPS, " groups and ", LPMM_BALANCE_TOKENS, " tokens in all are supported, got ", c.groups, " groups of ", c.tokens);
+    REQUIRE(c.tokens * c.picks < (int64_t)1 << 31, "fewer than 2^31 picks in a group are supported, got ", c.tokens, " tokens of ", c.picks);
     if (mask)
         REQUIRE(mask->scalar_type() == at::kBool && same_lead(*mask, router_logits, 0, 1), "mask must be a bool tensor of shape ",
                 router_logits.sizes().slice(0, dims - 1), ", got ", mask->scalar_type(), " of shape ", mask->sizes());

@@ -84,7 +84,7 @@ def balance_loss(router_logits, expert_ids, *, mask=None, weight=1.0, z_weight=0
 
     router_logits: (N, E) float32, float16 or bfloat16, or (G, N, E) for G groups (sequences, layers) that are balanced each by
     itself; E at most 1024, G at most 65535, G N at most 2^28.  expert_ids: (..., k) int32 or int64, the experts that each
-    token goes to, k at most E; a negative id is no pick (a token that was dropped).  mask: (...) bool, the tokens that take part.
+    token goes to, k at most E, N k below 2^31; a negative id is no pick (a token that was dropped).  mask: (...) bool, the tokens that take part.
 
     With p = softmax(router_logits), T a group's tokens that take part and c_e the picks of expert e among them, the loss is the mean
     over the groups of

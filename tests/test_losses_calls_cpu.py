@@ -140,3 +140,13 @@ def test_a_library_of_another_version_is_named_before_its_functions_are_looked_u
     monkeypatch.setattr(_native.ctypes, "CDLL", lambda path: Old())
     with pytest.raises(RuntimeError, match="ABI version 2, expected .*; rebuild it"):
         _native.lib()
+
+
+@pytest.mark.parametrize("tokens,picks", [(2 ** 28, 8), (2 ** 21, 1024)])
+def test_more_picks_than_31_bits_count_are_refused_by_name(tokens, picks):
+    r = torch.zeros(1, 1).expand(tokens, picks)
+    ids = torch.zeros(1, 1, dtype=torch.int32)
+    with pytest.raises(RuntimeError, match=f"fewer than 2\\^31 picks in a group are supported, got {tokens} tokens of {picks}"):
+        F.balance_loss(r, ids.expand(tokens, picks))
+    with pytest.raises(RuntimeError, match="CUDA"):
+        F.balance_loss(r, ids.expand(tokens, picks - 1))
