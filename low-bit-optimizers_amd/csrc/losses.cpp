@@ -335,6 +335,7 @@ Tensor distill_loss(const Tensor &logits, const Tensor &teacher_logits, const Te
     for (const int64_t n : logits.sizes().slice(0, logits.dim() - 1))
         c.rows *= n;
     REQUIRE(c.vocab >= 1 && c.vocab < (int64_t)1 << 31, "logits must have 1 to 2^31 - 1 values in their last dimension, got ", c.vocab);
+    REQUIRE(c.rows < (int64_t)1 << 31, "logits must have fewer than 2^31 rows, got ", c.rows);
     REQUIRE(c.topk <= LPMM_DISTILL_MOST, "at most ", LPMM_DISTILL_MOST, " teacher entries per row are supported, got ", c.topk);
     c.id_bits = id_bits(teacher_ids, "teacher_ids");
     c.teacher_group = group;

@@ -47,7 +47,7 @@ def distill_loss(logits, teacher_logits, teacher_ids, *, temperature=1.0, labels
                  ignore_index=-100, reduction="mean", teacher_quant=None):
     """Distillation from a teacher's top logits, differentiable in `logits`.
 
-    logits: (..., V) float32, float16 or bfloat16; views such as `logits[:, :-1]` are read in place.
+    logits: (..., V) float32, float16 or bfloat16, fewer than 2^31 rows; views such as `logits[:, :-1]` are read in place.
     teacher_logits, teacher_ids: (..., K), the teacher's K largest logits of each position and where in the vocabulary they
     are (int32 or int64), K at most 1024, in any order.  A negative id marks an empty entry.  The values are float32, float16 or
     bfloat16, or stored by `vectorwise_quant` with scale_type 'group' and 4 to 8 bits: then teacher_logits is

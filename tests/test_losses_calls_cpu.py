@@ -150,3 +150,14 @@ def test_more_picks_than_31_bits_count_are_refused_by_name(tokens, picks):
         F.balance_loss(r, ids.expand(tokens, picks))
     with pytest.raises(RuntimeError, match="CUDA"):
         F.balance_loss(r, ids.expand(tokens, picks - 1))
+
+
+def test_more_rows_than_31_bits_count_are_refused_by_name():
+    def call(rows):
+        x, ids = torch.zeros(1, 1).expand(rows, 1), torch.zeros(1, 0, dtype=torch.int64).expand(rows, 0)
+        return F.distill_loss(x, torch.zeros(1, 0).expand(rows, 0), ids)
+
+    with pytest.raises(RuntimeError, match="fewer than 2\\^31 rows, got 2147483648"):
+        call(2 ** 31)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        call(2 ** 31 - 1)
