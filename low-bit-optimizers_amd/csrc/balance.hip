@@ -23,6 +23,11 @@ namespace {
 
 constexpr int kBalThreads = 256, kBalWaves = kBalThreads / kWave, kLanes = 16;
 constexpr int kJoinThreads = 1024, kJoinColumns = 16;
+// Most probabilities that a thread adds in 32 bits, before doubles: one chain over all tokens of a long group drifts (identical tokens: after 2^14
+// additions by 1e-4 of the sum; after 128 by 8e-6 at most).  Doubles within the workgroup instead took registers: 19 -> 23 us at 65536 x 256 fp32,
+// 64 -> 94 at 1024 experts; 64 turns leave more to join (2^22 x 64 bf16: 33 us, with 128 turns 19, with chains of any length 11,
+// beside 225 of sums).
+constexpr int kBalTurns = 128;
 
 struct Balance {
     lpmm_balance_call c;
@@ -44,13 +49,19 @@ struct Split {
     int64_t parts, per, tiles;
 };
 
-// Tokens to a workgroup of the sums: 128 at least, so that what it joins at its end is little beside what it reads; 1024 workgroups at most,
-// four for each compute unit.  One workgroup alone joins its own sums, without a second launch.
+// Tokens to a workgroup of the sums: 128 at least, so that what it joins at its end is little beside what it reads; 1024 workgroups, four for
+// each compute unit, unless a thread would then add more than kBalTurns tokens' probabilities in 32 bits.  One workgroup alone joins its own
+// sums, without a second launch.
 Split split(int64_t groups, int64_t tokens, int64_t experts)
 {
+    int64_t lanes = 1;  // to a token of float32; 16-bit types may have half as many, and half as many turns
+    while (lanes < kLanes && lanes * F32::kRun < experts)
+        lanes *= 2;
+    const int64_t longest = kBalTurns * (kBalThreads / lanes), least = (tokens + longest - 1) / longest;
     const int64_t most = groups >= 1024 ? 1 : 1024 / groups;
     int64_t parts = (tokens + 127) / 128;
-    parts = parts > most ? most : parts < 1 ? 1 : parts;
+    parts = parts > most ? most : parts;
+    parts = parts < least ? least : parts < 1 ? 1 : parts;
     return {parts, (tokens + parts - 1) / parts, (experts + kJoinColumns - 1) / kJoinColumns};
 }
 
@@ -164,7 +175,7 @@ __device__ __forceinline__ void join(const Balance &a, int64_t group, int tile, 
     const int64_t base = group * a.parts;
     double square = 0.0, prob = 0.0;
     int seen = 0;
-    if (tid < a.parts) {  // at most as many as the workgroup has threads: split
+    if (tid < a.parts) {  // asked for before the parts of the experts; long groups have more
         square = a.square[base + tid];
         seen = a.seen[base + tid];
     }
@@ -179,6 +190,14 @@ __device__ __forceinline__ void join(const Balance &a, int64_t group, int tile, 
                     picked += a.picked[at];
                 }
     }
+    bool wrong_ids = seen < 0;
+    seen = seen < 0 ? -1 - seen : seen;
+    for (int64_t p = tid + THREADS; p < a.parts; p += THREADS) {
+        const int n = a.seen[base + p];
+        square += a.square[base + p];
+        seen += n < 0 ? -1 - n : n;  // all together at most 2^28
+        wrong_ids |= n < 0;
+    }
     double count = (double)picked;  // exact
 #pragma unroll
     for (int o = kJoinColumns; o < kWave; o <<= 1) {
@@ -186,8 +205,8 @@ __device__ __forceinline__ void join(const Balance &a, int64_t group, int tile, 
         count += __shfl_xor(count, o, kWave);
     }
     square = wave_sum_f64(square);
-    double tokens = wave_sum_f64((double)(seen < 0 ? -1 - seen : seen));
-    const bool any_wrong = __any(seen < 0);
+    double tokens = wave_sum_f64((double)seen);
+    const bool any_wrong = __any(wrong_ids);
     if (lane < kJoinColumns)
         room.prob[wave][lane] = prob, room.count[wave][lane] = count;
     if (lane == 0)
