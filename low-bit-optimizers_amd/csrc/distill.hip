@@ -30,6 +30,7 @@ enum Shared {
     kCountHere,  // few rows: every workgroup counts them, a microsecond each at once, for a launch less
 };
 constexpr int64_t kFewRows = 256;  // at most a workgroup's threads
+constexpr int kChain = 128;  // values whose exponentials a thread adds in 32 bits
 constexpr int64_t kMostRows = (int64_t)1 << 21;  // of a launch, whose threads are counted in 32 bits
 
 struct Distill {
@@ -403,6 +404,26 @@ __global__ __launch_bounds__(THREADS, WAVES) void distill_kernel(Distill a)
             read_runs(body);
         }
     };
+    // adds the exponentials of all runs.  Rows that are held are 128 additions to a thread; longer ones are read, and their chains of 32-bit
+    // additions end after as many (2^14, of a row of 2^24 values that are alike, are off by 1e-4)
+    auto read_sums = [&](auto one_step, const Shift &t, const Shift &one, Sums &s) {
+        constexpr bool kInOne = decltype(one_step)::value;
+        if constexpr (RUNS > 0) {
+            read_runs([&](uint32_t, u32x4 r) { run_sums<T, KIND, kInOne>(r, t, one, s.sum, s.sum1); });
+        } else {
+            double sum = s.sum, sum1 = s.sum1;
+            for (uint32_t at = first; at < cut.end;) {
+                float near = 0.0f, near1 = 0.0f;
+#pragma unroll 1
+                for (int n = 0; n < kChain / T::kRun && at < cut.end; ++n, at += kStride)
+                    run_sums<T, KIND, kInOne>(load_run<T>(x + at), t, one, near, near1);
+                sum += (double)near;
+                sum1 += (double)near1;
+            }
+            s.sum = (float)sum;
+            s.sum1 = (float)sum1;
+        }
+    };
     const float alone = single < vocab ? from_bits<T>(alone_bits) : -INFINITY;
     const float ct = KIND == kOne && c.temperature == 1.0f ? kLog2e : kLog2e / c.temperature;
     const float inv_t = 1.0f / c.temperature;
@@ -441,7 +462,10 @@ __global__ __launch_bounds__(THREADS, WAVES) void distill_kernel(Distill a)
         shifts<T, KIND>(s.max, ct, t, one);
         s.sum = exp2_fast(kOneStep ? fmaf(alone, t.c, -t.m) : (alone - t.max) * t.c);
         s.sum1 = KIND == kSquare ? s.sum * s.sum : KIND == kTwo ? exp2_fast(kOneStep ? fmaf(alone, one.c, -one.m) : (alone - one.max) * one.c) : 0.0f;
-        runs([&](uint32_t, u32x4 r) { run_sums<T, KIND, kOneStep>(r, t, one, s.sum, s.sum1); });
+        if constexpr (RUNS > 0)
+            runs([&](uint32_t, u32x4 r) { run_sums<T, KIND, kOneStep>(r, t, one, s.sum, s.sum1); });
+        else
+            read_sums(std::bool_constant<kOneStep>(), t, one, s);
         // s.sum is NaN where t.m is: values too large for one step
         const bool fit = !(none && first < cut.end) && s.sum < 0x1p30f && (KIND != kTwo || s.sum1 < 0x1p30f);
         const float most = wave_max(s.sum == 0.0f ? -INFINITY : s.max);
@@ -476,9 +500,9 @@ __global__ __launch_bounds__(THREADS, WAVES) void distill_kernel(Distill a)
             s.sum = exp2_fast(t.of_value(alone));
             s.sum1 = KIND == kSquare ? s.sum * s.sum : KIND == kTwo ? exp2_fast(one.of_value(alone)) : 0.0f;
             if (kOneStep && t.one_step())
-                read_runs([&](uint32_t, u32x4 r) { run_sums<T, KIND, kOneStep>(r, t, one, s.sum, s.sum1); });
+                read_sums(std::bool_constant<kOneStep>(), t, one, s);
             else
-                read_runs([&](uint32_t, u32x4 r) { run_sums<T, KIND, false>(r, t, one, s.sum, s.sum1); });
+                read_sums(std::false_type(), t, one, s);
             s.sum = wave_sum(s.sum);
             if (KIND != kOne)
                 s.sum1 = wave_sum(s.sum1);

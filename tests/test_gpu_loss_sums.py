@@ -144,3 +144,28 @@ def test_every_value_of_a_row_is_counted_once(rows, dtype):
     for vocab in (777, 9001, 50257, 137 * run * 1024 // 8 + 5):
         _exact_distill(rows, vocab, dtype, 0.5, 1.5, 0.5, 0.25)
         _exact_distill(rows, vocab, dtype, 0.001, 1.0, 1.0, 0.5)  # most first runs say nothing of the rest
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("temperature", [1.0, 1.5])
+def test_rows_of_millions_of_values(dtype, temperature):
+    """2^24 values that are alike but for every thread's first: 16384 to a thread, in which one chain of 32-bit additions drifts by 1e-4."""
+    vocab, low = (1 << 24) + 5, -4.28125
+    x = torch.full((1, vocab), low, device="cuda", dtype=dtype)
+    x[:, : 1024 * 8 + 16] = 0.0
+    x[:, -9:] = 0.0
+    x.requires_grad_(True)
+    label = torch.tensor([vocab // 2], device="cuda")
+    entry = torch.tensor([[5]], device="cuda")
+    loss = F.distill_loss(x, torch.zeros(1, 1, device="cuda"), entry, temperature=temperature, labels=label, teacher_weight=1.0, label_weight=0.5)
+    grad = torch.autograd.grad(loss, x)[0]
+    n = 1024 * 8 + 16 + 9
+    some = torch.tensor([0.0, low], dtype=torch.float64)
+    sums = [(n + (vocab - n) * torch.exp(some[1] / t)) for t in (temperature, 1.0)]
+    want = temperature ** 2 * sums[0].log() + 0.5 * (sums[1].log() - low)
+    # a term of the sum: three roundings of its exponent and two half steps; 128 additions in a thread, 6 and 10 to join
+    off = U * (3 * -low / min(temperature, 1.0) + 2 + 128 + 16)
+    ref.assert_within(loss, want, (temperature ** 2 + 0.5) * off + 8 * U * want, "loss")
+    for at, v in ((vocab // 3, low), (100, 0.0)):
+        q = temperature * torch.exp(torch.tensor(v / temperature).double()) / sums[0] + 0.5 * torch.exp(torch.tensor(v).double()) / sums[1]
+        ref.assert_within(grad[0, at], q, q * (off + U * (3 * -low / min(temperature, 1.0) + 10)), f"gradient of {v}")
