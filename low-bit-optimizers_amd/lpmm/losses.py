@@ -47,7 +47,9 @@ def distill_loss(logits, teacher_logits, teacher_ids, *, temperature=1.0, labels
                  ignore_index=-100, reduction="mean", teacher_quant=None):
     """Distillation from a teacher's top logits, differentiable in `logits`.
 
-    logits: (..., V) float32, float16 or bfloat16, fewer than 2^31 rows; views such as `logits[:, :-1]` are read in place.
+    logits: (..., V) float32, float16 or bfloat16, fewer than 2^31 rows; views are read in place.  For next tokens pass whole logits and
+    shifted labels whose last one is ignore_index: `logits[:, :-1]` is the same loss, but the slice's backward pass writes all of
+    the gradient twice more (4 x 2048 x 32000 bf16: 504 us for loss and gradient, 199 from whole logits).
     teacher_logits, teacher_ids: (..., K), the teacher's K largest logits of each position and where in the vocabulary they
     are (int32 or int64), K at most 1024, in any order.  A negative id marks an empty entry.  The values are float32, float16 or
     bfloat16, or stored by `vectorwise_quant` with scale_type 'group' and 4 to 8 bits: then teacher_logits is
@@ -65,8 +67,8 @@ def distill_loss(logits, teacher_logits, teacher_ids, *, temperature=1.0, labels
     ignore_index (whatever its weight), and teacher values of NaN or +infinity make the loss and the gradient of their row NaN.
 
     Returns a float32 tensor: a scalar for reduction 'mean' or 'sum', (...) for 'none'.  No gradient flows to the teacher.  With
-    'mean' and 'sum' factors are best put into the two weights: the gradient is then made along with the loss, while a loss
-    that is multiplied afterwards has it written once more."""
+    'mean' and 'sum' factors are best put into the two weights: the gradient of float32 and bfloat16 logits is then made along with the
+    loss, while a loss that is multiplied afterwards has it written once more (378 us instead of 199)."""
     if reduction not in _REDUCTIONS:
         raise ValueError(f"reduction must be one of {sorted(_REDUCTIONS)}, got {reduction!r}")
     scale, qmap, group, bits = (None, None, 1, 8) if teacher_quant is None else _stored_teacher(teacher_quant)

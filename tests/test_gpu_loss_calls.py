@@ -90,3 +90,56 @@ def test_a_compiled_step_runs_the_call_as_it_is(make):
     assert torch.equal(got.detach(), want.detach())
     a, b = torch.autograd.grad(got, x)[0], torch.autograd.grad(want, x)[0]
     assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("with_label", [True, False])
+def test_labels_that_leave_the_last_position_out(dtype, with_label):
+    """Whole logits with shifted labels are the loss of the slice, in 64 bits and as the package computes the slice."""
+    import losses_ref as ref
+
+    g = torch.Generator().manual_seed(3)
+    x = (torch.randn(3, 9, 67, generator=g) * 3).to(dtype)
+    t, ids = torch.randn(3, 9, 6, generator=g) * 3, torch.randint(-1, 67, (3, 9, 6), generator=g)
+    tokens = torch.randint(0, 67, (3, 9), generator=g)
+    shifted = torch.nn.functional.pad(tokens[:, 1:], (0, 1), value=-100)
+    kw = dict(temperature=2.0, teacher_weight=0.75, label_weight=0.5 if with_label else 0.0)
+    leaf, view = x.cuda().requires_grad_(True), x.cuda().requires_grad_(True)
+    F.distill_loss(leaf, t.cuda(), ids.cuda(), labels=shifted.cuda(), **kw).backward()
+    loss = F.distill_loss(leaf, t.cuda(), ids.cuda(), labels=shifted.cuda(), **kw)
+    sliced = F.distill_loss(view[:, :-1], t[:, :-1].cuda(), ids[:, :-1].cuda(), labels=tokens[:, 1:].cuda() if with_label else None, **kw)
+    sliced.backward()
+    want, bound, grad, gbound = ref.distill(x[:, :-1], t[:, :-1], ids[:, :-1], 2.0, tokens[:, 1:] if with_label else None, 0.75, kw["label_weight"])
+    ref.assert_within(loss, want, bound, "whole")
+    ref.assert_within(sliced, want, bound, "slice")
+    ref.assert_within(leaf.grad[:, :-1], grad, gbound, "whole gradient")
+    ref.assert_within(view.grad[:, :-1], grad, gbound, "slice gradient")
+    assert not leaf.grad[:, -1].any() and not view.grad[:, -1].any()
+
+
+def test_the_documented_step():
+    """Teacher stored offline, whole logits, labels that leave the last position out, the balance beside it, one backward pass."""
+    import losses_ref as ref
+
+    g = torch.Generator().manual_seed(4)
+    teacher, tokens = (torch.randn(2, 33, 301, generator=g) * 3).cuda(), torch.randint(0, 301, (2, 33), generator=g)
+    top = teacher.topk(16, dim=-1)
+    kw = dict(b=8, signed=True, quant_type="power-1", round_type="real-nearest", scale_type="group", gp_sz=128,
+              qmap=F.create_general_qmap("power-1", 8, True).cuda())
+    codes, md = F.vectorwise_quant((top.values - top.values[..., :1]).float(), **kw)
+    back = F.vectorwise_dequant(codes, shape=top.values.shape, **kw, **md).cpu()
+    shifted = torch.nn.functional.pad(tokens[:, 1:], (0, 1), value=-100)
+    x, r = torch.randn(2, 33, 301, generator=g) * 2, torch.randn(66, 12, generator=g)
+    picks = r.topk(2, dim=-1).indices
+    logits, router = x.cuda().requires_grad_(True), r.cuda().requires_grad_(True)
+    loss = F.distill_loss(logits, codes, top.indices, temperature=2.0, labels=shifted.cuda(), teacher_weight=0.5, label_weight=0.5,
+                          teacher_quant=dict(kw, **md))
+    aux, counts = F.balance_loss(router, picks.cuda(), weight=0.01, z_weight=0.001)
+    (loss + aux).backward()
+    want, bound, grad, gbound = ref.distill(x, back, top.indices.cpu(), 2.0, shifted, 0.5, 0.5)
+    ref.assert_within(loss, want, bound, "loss")
+    ref.assert_within(logits.grad, grad, gbound, "gradient")
+    want, bound, wcounts, grad, gbound = ref.balance(r, picks, None, 0.01, 0.001)
+    ref.assert_within(aux, want, bound, "balance")
+    ref.assert_within(router.grad, grad, gbound, "its gradient")
+    assert torch.equal(counts.cpu(), wcounts)
