@@ -3,8 +3,9 @@
 // With p = softmax(r) of a token, c_e the picks of expert e, T tokens and k picks a token in a group of tokens:
 //     loss_g = w E sum_e c_e / (T k) * (1/T) sum_n p_ne + z / T sum_n lse_n^2        loss = 1/G sum_g loss_g
 //     d loss / d r_ne = p_ne (f_e - sum_j f_j p_nj + h lse_n),  f_e = w E c_e / (T^2 k G),  h = 2 z / (T G)
-// The gradient needs the counts of the whole group, so the logits are read twice: by the call that sums the probabilities and counts the
-// picks, and by the one that writes the gradient, which makes the probabilities again rather than read them back (4 bytes a value).
+// The logits are read twice: by the call that sums the probabilities and counts the picks, and by the one that writes the gradient, which makes the
+// probabilities again rather than read them back (4 bytes a value).  The gradient needs the counts of the whole group.  These depend on ids and
+// masks alone, so that counting first would let one pass over the logits give loss and gradient; that form is not built.
 //
 // A token's logits lie across up to 16 neighbouring lanes, in chunks of 16 bytes a lane, so that its maximum and its sums are exchanges
 // within a row of lanes (no shared memory) and every load of a wave covers whole stretches of several tokens.  A thread keeps the sums of
