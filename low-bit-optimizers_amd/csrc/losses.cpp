@@ -127,12 +127,13 @@ c10::Device device_of(std::initializer_list<Named> tensors)
 const Tensor *some(const MaybeTensor &t) { return t ? &*t : nullptr; }
 Tensor or_none(const MaybeTensor &t) { return t ? *t : Tensor(); }
 
-// Constants of the loss: contiguous, and without a graph of their own.
+// Constants of the loss: contiguous, without a graph of their own, and with the signs they stand for (torch negates some views, such as
+// the imaginary part of a conjugate, only where they are read).
 Tensor constant(const Tensor &t)
 {
     if (!t.defined())
         return t;
-    const Tensor plain = t.requires_grad() ? t.detach() : t;
+    const Tensor plain = (t.requires_grad() ? t.detach() : t).resolve_neg();
     return plain.is_contiguous() ? plain : plain.contiguous();
 }
 
@@ -223,7 +224,9 @@ struct Kept {
     // also checks that nothing was written over since the loss was computed
     Tensor back(c10::Device device) const
     {
-        const Tensor t = variable.unpack();
+        Tensor t = variable.unpack();
+        if (t.defined())
+            t = t.resolve_neg();
         REQUIRE(!some || (t.defined() && t.device() == device && t.scalar_type() == type && t.sizes() == shape), "a saved tensor of ", type, ", shape ",
                 at::IntArrayRef(shape), " on ", device, " came back from its hooks as another");
         return t;
@@ -257,10 +260,10 @@ struct DistillLossBackward : public Node {
     variable_list apply(variable_list &&grads) override
     {
         std::lock_guard<std::mutex> lock(mutex_);
-        Tensor grad_loss = grads[0];
-        if (!grad_loss.defined())
+        if (!grads[0].defined())
             return {Tensor()};
-        require_seen(grad_loss, "the gradient of the loss", "distill_loss");
+        require_seen(grads[0], "the gradient of the loss", "distill_loss");
+        Tensor grad_loss = grads[0].resolve_neg();
         const c10::DeviceGuard guard(device);
         Tensor x = rows.back(device);
         std::optional<Rows> strides = row_strides(x);
@@ -367,8 +370,8 @@ Tensor distill_loss(const Tensor &logits, const Tensor &teacher_logits, const Te
 
     std::optional<Rows> strides = row_strides(logits);
     Tensor rows = logits;
-    if (!strides) {
-        rows = logits.detach().contiguous();
+    if (!strides || logits.is_neg()) {
+        rows = logits.detach().resolve_neg().contiguous();
         strides = row_strides(rows);
     }
     c.inner = strides->inner;
@@ -377,12 +380,13 @@ Tensor distill_loss(const Tensor &logits, const Tensor &teacher_logits, const Te
     c.ignore_index = ignore_index;
     c.reduction = reduction;
     const Tensor teacher = constant(teacher_logits), ids = constant(teacher_ids), y = constant(or_none(labels));
+    const Tensor scales = constant(or_none(scale)), map = constant(or_none(qmap));
     c.logits = rows.data_ptr();
     c.teacher = teacher.data_ptr();
     c.ids = ids.data_ptr();
     c.labels = data<int64_t>(y);
-    c.teacher_scale = scale ? data<float>(*scale) : nullptr;
-    c.teacher_map = qmap ? data<float>(*qmap) : nullptr;
+    c.teacher_scale = data<float>(scales);
+    c.teacher_map = data<float>(map);
 
     const bool none = reduction == LPMM_REDUCE_NONE;
     const at::TensorOptions floats = at::TensorOptions().dtype(at::kFloat).device(device);
@@ -413,8 +417,8 @@ Tensor distill_loss(const Tensor &logits, const Tensor &teacher_logits, const Te
     node->teacher.keep(teacher);
     node->ids.keep(ids);
     node->labels.keep(y);
-    node->scale.keep(or_none(scale));
-    node->map.keep(or_none(qmap));
+    node->scale.keep(scales);
+    node->map.keep(map);
     node->work.keep(work);
     node->recorded = grad.defined() ? recording(stream_of(device)) : 0;
     node->grad = std::move(grad);
@@ -443,6 +447,7 @@ struct BalanceLossBackward : public Node {
         if (x.stride(-1) != 1)
             x = x.contiguous();
         const Tensor seen = mask.back_contiguous(device), f = factors.back_contiguous(device);
+        const Tensor grad_loss = grads[0].resolve_neg();
         Tensor out = at::empty(shape, options);
         lpmm_balance_call c = call;
         c.logits = x.data_ptr();
@@ -454,7 +459,7 @@ struct BalanceLossBackward : public Node {
         c.counts = nullptr;
         c.loss = nullptr;
         c.grad = out.data_ptr();
-        check(lpmm_balance_loss_grad(&c, static_cast<const float *>(grads[0].data_ptr()), stream_of(device)), "balance_loss_grad");
+        check(lpmm_balance_loss_grad(&c, static_cast<const float *>(grad_loss.data_ptr()), stream_of(device)), "balance_loss_grad");
         return {once(std::move(out), next_edge(0), "balance_loss")};
     }
 
@@ -497,8 +502,8 @@ std::pair<Tensor, Tensor> balance_loss(const Tensor &router_logits, const Tensor
     const bool wants_grad = router_logits.requires_grad() && c10::GradMode::is_enabled();
 
     Tensor rows = router_logits;
-    if (rows.stride(-1) != 1 && c.experts > 1)
-        rows = rows.detach().contiguous();
+    if ((rows.stride(-1) != 1 && c.experts > 1) || rows.is_neg())
+        rows = rows.detach().resolve_neg().contiguous();
     c.outer_stride = dims == 3 ? rows.stride(0) : 0;
     c.inner_stride = rows.stride(-2);
     const Tensor ids = constant(expert_ids), seen = constant(or_none(mask));

@@ -143,3 +143,36 @@ def test_the_documented_step():
     ref.assert_within(aux, want, bound, "balance")
     ref.assert_within(router.grad, grad, gbound, "its gradient")
     assert torch.equal(counts.cpu(), wcounts)
+
+
+@pytest.mark.parametrize("make", BOTH)
+def test_a_gradient_that_is_negated_where_it_is_read(make):
+    """What complex arithmetic behind the loss sends back may be the imaginary part of a conjugate, whose memory has the other sign."""
+    x, loss = make()
+    plain = torch.autograd.grad(loss(), x)[0]
+    seen = []
+    value = loss()
+    value.register_hook(lambda g: seen.append(g.is_neg()))
+    grad = torch.autograd.grad((torch.complex(torch.ones((), device="cuda"), value).conj() * (2 + 3j)).imag, x)[0]
+    assert seen == [True]
+    assert ((grad + 2 * plain).abs() <= 4 * 2.0 ** -24 * grad.abs() + 2.0 ** -126).all()  # two roundings of a product on either side
+
+
+def test_inputs_that_are_negated_where_they_are_read():
+    x, _ = _distill()
+    g = torch.Generator().manual_seed(1)
+    ids = torch.randint(0, 300, (6, 5), generator=g).cuda()
+    t = torch.randn(6, 5, generator=g).cuda()
+    for neg in (lambda a: torch._neg_view(-a), lambda a: torch.complex(a, -a).conj().imag):
+        other = neg(x.detach())
+        assert other.is_neg()
+        want, got = (F.distill_loss(a, b, ids, temperature=2.0) for a, b in ((x.detach(), t), (other, neg(t))))
+        assert torch.equal(want, got)
+        leaf = neg(x.detach()).requires_grad_(True)
+        grads = [torch.autograd.grad(F.distill_loss(a, t, ids), a)[0] for a in (x, leaf)]
+        assert torch.equal(*grads)
+    router, picks = torch.randn(40, 12, generator=g).cuda(), torch.randint(0, 12, (40, 2), generator=g).cuda()
+    leaves = [router.clone().requires_grad_(True), torch._neg_view(-router).requires_grad_(True)]
+    both = [F.balance_loss(a, picks, z_weight=0.1)[0] for a in leaves]
+    assert torch.equal(both[0].detach(), both[1].detach())
+    assert torch.equal(*[torch.autograd.grad(b, a)[0] for b, a in zip(both, leaves)])
