@@ -104,6 +104,9 @@ void require_seen(const Tensor &t, const char *name, const char *what)
     REQUIRE(!t._fw_grad(0).defined(), name, " has a forward-mode gradient, and ", what, " has no forward-mode derivative");
 }
 
+// Not so of tensors that wrap others: their address is NULL, which for labels and masks would read as none.
+bool has_memory(const Tensor &t) { return t.numel() == 0 || t.const_data_ptr(); }
+
 struct Named {
     const Tensor *tensor;
     const char *name;
@@ -119,7 +122,7 @@ c10::Device device_of(std::initializer_list<Named> tensors)
         if (!device)
             device = t.tensor->device();
         REQUIRE(t.tensor->device() == *device, "all tensors must be on the same device, got ", *device, " and ", t.tensor->device());
-        REQUIRE(t.tensor->numel() == 0 || t.tensor->const_data_ptr(), t.name, " has no memory of its own: a tensor that wraps others is not taken");
+        REQUIRE(has_memory(*t.tensor), t.name, " has no memory of its own: a tensor that wraps others is not taken");
     }
     return *device;
 }
@@ -227,7 +230,7 @@ struct Kept {
         Tensor t = variable.unpack();
         if (t.defined())
             t = t.resolve_neg();
-        REQUIRE(!some || (t.defined() && t.device() == device && t.scalar_type() == type && t.sizes() == shape), "a saved tensor of ", type, ", shape ",
+        REQUIRE(!some || (t.defined() && t.device() == device && t.scalar_type() == type && t.sizes() == shape && has_memory(t)), "a saved tensor of ", type, ", shape ",
                 at::IntArrayRef(shape), " on ", device, " came back from its hooks as another");
         return t;
     }

@@ -176,3 +176,30 @@ def test_inputs_that_are_negated_where_they_are_read():
     both = [F.balance_loss(a, picks, z_weight=0.1)[0] for a in leaves]
     assert torch.equal(both[0].detach(), both[1].detach())
     assert torch.equal(*[torch.autograd.grad(b, a)[0] for b, a in zip(both, leaves)])
+
+
+class _Wraps(torch.Tensor):
+    @staticmethod
+    def __new__(cls, inner):
+        return torch.Tensor._make_wrapper_subclass(cls, inner.shape, dtype=inner.dtype, device=inner.device, strides=inner.stride())
+
+    @classmethod
+    def __torch_dispatch__(cls, func, types, args=(), kwargs=None):
+        raise AssertionError(f"{func} of a wrapper")
+
+
+@pytest.mark.parametrize("make,wrapped", [(_distill, torch.int64), (_balance, torch.bool)])
+def test_saved_tensors_that_come_back_without_memory_are_refused(make, wrapped):
+    """Labels and masks above all: an address of NULL means that there are none."""
+    if make is _balance:
+        x = torch.randn(40, 12, device="cuda", requires_grad=True)
+        ids, mask = torch.randint(0, 12, (40, 2), device="cuda"), torch.rand(40, device="cuda") < 0.5
+
+        def loss():
+            return F.balance_loss(x, ids, mask=mask)[0]
+    else:
+        x, loss = make()
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t, lambda t: _Wraps(t) if t.dtype == wrapped else t):
+        value = loss()
+    with pytest.raises(RuntimeError, match="came back from its hooks as another"):
+        value.backward()
