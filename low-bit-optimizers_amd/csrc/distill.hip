@@ -532,7 +532,15 @@ __global__ __launch_bounds__(THREADS, WAVES) void distill_kernel(Distill a)
         if (has_entry)
             part[tid] = kt * p;
         if (!AGAIN) {
-            const float kd = wave_sum(p > 0.0f ? p * ((z - log_total) - (t.of_value(from_bits<T>(entry.x)) * kLn2 - log_s)) : 0.0f);
+            float kd = 0.0f;
+            if (p > 0.0f) {
+                const float value = from_bits<T>(entry.x), e = t.of_value(value), weight = c.teacher_weight * c.temperature;
+                if (e != -INFINITY)
+                    kd = p * ((z - log_total) - (e * kLn2 - log_s)) * (weight * c.temperature);
+                else  // a logit that far below the others has no exponent of 2 in float32, but a loss: T^2 (x - max) / T
+                    kd = p * ((z - log_total) + log_s) * (weight * c.temperature) - (p * weight * value - p * weight * all.max);
+            }
+            kd = wave_sum(kd);
             if (tid % kWave == 0)
                 room[wave].kd = kd;
         }
@@ -563,9 +571,13 @@ __global__ __launch_bounds__(THREADS, WAVES) void distill_kernel(Distill a)
         float loss = 0.0f;
         for (int w = 0; w < kWaves && w * kWave < topk; ++w)
             loss += room[w].kd;
-        loss *= c.teacher_weight * (c.temperature * c.temperature);
-        if (a.with_label)
-            loss += c.label_weight * (logf(all.sum1) - one.of_value(from_bits<T>(label_bits)) * kLn2);
+        if (a.with_label) {
+            const float value = from_bits<T>(label_bits), e = one.of_value(value), log_s1 = logf(all.sum1);
+            if (e != -INFINITY)
+                loss += c.label_weight * (log_s1 - e * kLn2);
+            else
+                loss += c.label_weight * log_s1 - (c.label_weight * value - c.label_weight * all.max);
+        }
         c.row_loss[row] = bad ? NAN : loss;
     }
     if (!grad)

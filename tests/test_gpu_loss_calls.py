@@ -203,3 +203,32 @@ def test_saved_tensors_that_come_back_without_memory_are_refused(make, wrapped):
         value = loss()
     with pytest.raises(RuntimeError, match="came back from its hooks as another"):
         value.backward()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("temperature", [0.25, 1.0, 1.25, 2.0])
+def test_entries_and_labels_at_masked_logits_of_the_lowest_value(dtype, temperature):
+    """Their losses are large and not infinite: a logit of -3.4e38 has an exponent of 2 that float32 has not."""
+    import losses_ref as ref
+
+    g = torch.Generator().manual_seed(5)
+    least, most = torch.finfo(dtype).min, torch.finfo(dtype).max
+    for vocab in (203, 9001):
+        x = (torch.randn(6, vocab, generator=g) * 2).to(dtype)
+        t, y = torch.randn(6, 5, generator=g), torch.randint(100, 200, (6,), generator=g)
+        ids = torch.arange(5).expand(6, 5) * 17 + 3
+        x[0, 20] = least  # an entry
+        x[1, y[1]] = least  # the label
+        x[2, 20], x[2, y[2]] = least, least
+        x[3, 1] = most  # all but one
+        x[4, 1], x[4, 20], x[4, y[4]] = most, least, least
+        for wt, wl in ((0.125, 0.125), (0.125, 0.0), (0.0, 0.125)):
+            kw = dict(temperature=temperature, teacher_weight=wt, label_weight=wl, reduction="none")
+            leaf = x.cuda().requires_grad_(True)
+            loss = F.distill_loss(leaf, t.cuda(), ids.cuda(), labels=y.cuda(), **kw)
+            up = 1024.0 if dtype == torch.float16 else 1.0
+            grad = torch.autograd.grad(loss, leaf, torch.full((6,), up, device="cuda"))[0]
+            want, bound, wgrad, gbound = ref.distill(x, t, ids, temperature, y, wt, wl, reduction="none", grad_loss=torch.full((6,), up))
+            assert want.lt(torch.finfo(torch.float32).max).all()
+            ref.assert_within(loss, want, bound, f"{vocab} {wt} {wl} loss")
+            ref.assert_within(grad, wgrad, gbound, f"{vocab} {wt} {wl} gradient")
