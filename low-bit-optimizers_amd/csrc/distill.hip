@@ -535,7 +535,7 @@ __global__ __launch_bounds__(THREADS, WAVES) void distill_kernel(Distill a)
             float kd = 0.0f;
             if (p > 0.0f) {
                 const float value = from_bits<T>(entry.x), e = t.of_value(value), weight = c.teacher_weight * c.temperature;
-                if (e != -INFINITY)
+                if (e != -INFINITY || value == -INFINITY)
                     kd = p * ((z - log_total) - (e * kLn2 - log_s)) * (weight * c.temperature);
                 else  // a logit that far below the others has no exponent of 2 in float32, but a loss: T^2 (x - max) / T
                     kd = p * ((z - log_total) + log_s) * (weight * c.temperature) - (p * weight * value - p * weight * all.max);
@@ -573,7 +573,7 @@ __global__ __launch_bounds__(THREADS, WAVES) void distill_kernel(Distill a)
             loss += room[w].kd;
         if (a.with_label) {
             const float value = from_bits<T>(label_bits), e = one.of_value(value), log_s1 = logf(all.sum1);
-            if (e != -INFINITY)
+            if (e != -INFINITY || value == -INFINITY)
                 loss += c.label_weight * (log_s1 - e * kLn2);
             else
                 loss += c.label_weight * log_s1 - (c.label_weight * value - c.label_weight * all.max);

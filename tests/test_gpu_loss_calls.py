@@ -232,3 +232,18 @@ def test_entries_and_labels_at_masked_logits_of_the_lowest_value(dtype, temperat
             assert want.lt(torch.finfo(torch.float32).max).all()
             ref.assert_within(loss, want, bound, f"{vocab} {wt} {wl} loss")
             ref.assert_within(grad, wgrad, gbound, f"{vocab} {wt} {wl} gradient")
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+def test_entries_of_little_probability_at_masked_logits(dtype):
+    """Whatever the teacher gives to a logit of -infinity, the smallest numbers that float32 has among it, the loss is infinite and not NaN."""
+    for weight, temperature in ((1.0, 1.0), (1e-3, 1.0), (0.25, 0.25), (-0.5, 2.0)):
+        x = torch.zeros(4, 40, dtype=dtype)
+        x[:, 7] = -float("inf")
+        t = torch.zeros(4, 3)
+        t[:, 1] = torch.tensor([-1.0, -60.0, -92.0, -100.0]) * temperature  # e^-100: 4e-44, which a weight takes to 0
+        ids, y = torch.tensor([3, 7, 5]).expand(4, 3), torch.tensor([0, 1, 7, 2])
+        loss = F.distill_loss(x.cuda(), t.cuda(), ids.cuda(), temperature=temperature, teacher_weight=weight, reduction="none")
+        assert loss.isinf().all() and (loss * weight > 0).all()
+        loss = F.distill_loss(x.cuda(), t.cuda(), ids.cuda(), labels=y.cuda(), teacher_weight=0.0, label_weight=abs(weight), reduction="none")
+        assert loss.isinf().tolist() == [False, False, True, False] and loss[2] > 0
