@@ -29,6 +29,9 @@ constexpr int kJoinThreads = 1024, kJoinColumns = 16;
 // 64 -> 94 at 1024 experts; 64 turns leave more to join (2^22 x 64 bf16: 33 us, with 128 turns 19, with chains of any length 11,
 // beside 225 of sums).
 constexpr int kBalTurns = 128;
+// The gradient's factors are kept divided by this, and grad_loss is multiplied by it: the same bits in the end, but h lse alone would leave float32 where
+// logits are of its largest or lowest values and h is 1 or 2 (a group of few tokens), and infinity times a probability of 0 is NaN.
+constexpr float kLift = 16.0f;
 
 struct Balance {
     lpmm_balance_call c;
@@ -230,13 +233,13 @@ __device__ __forceinline__ void join(const Balance &a, int64_t group, int tile, 
         if (lane < kJoinColumns && e < experts) {
             const double share = c.picks > 0 ? (double)c.weight * experts * per * per / (double)c.picks : 0.0;
             c.counts[group * experts + e] = (int64_t)count;
-            c.factors[group * (experts + 2) + e] = wrong ? NAN : (float)(share * count / (double)c.groups);
+            c.factors[group * (experts + 2) + e] = wrong ? NAN : (float)(share * count / (double)c.groups / kLift);
             loss = share * count * prob;
         }
         loss = wave_sum_f64(loss);
         if (lane == 0) {
             if (tile == 0) {
-                c.factors[group * (experts + 2) + experts] = (float)(2.0 * (double)c.z_weight * per / (double)c.groups);
+                c.factors[group * (experts + 2) + experts] = (float)(2.0 * (double)c.z_weight * per / (double)c.groups / kLift);
                 c.factors[group * (experts + 2) + experts + 1] = 0.0f;
                 loss = wrong ? NAN : loss + (double)c.z_weight * square * per;
             }
@@ -383,7 +386,7 @@ __global__ __launch_bounds__(kBalThreads) void balance_grad_kernel(Balance a)
     bool now = takes(begin + tid / a.lanes);
     load_logits<T, CHUNKS>(logits + (begin + tid / a.lanes) * c.inner_stride, place, now, raw);
     const float *factors = c.factors + group * (experts + 2);
-    const float scale = a.grad_loss[0], h = factors[experts];
+    const float scale = a.grad_loss[0] * kLift, h = factors[experts];
     float f[CHUNKS][kRun];
 #pragma unroll
     for (int i = 0; i < CHUNKS; ++i)

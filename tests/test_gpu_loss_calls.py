@@ -247,3 +247,26 @@ def test_entries_of_little_probability_at_masked_logits(dtype):
         assert loss.isinf().all() and (loss * weight > 0).all()
         loss = F.distill_loss(x.cuda(), t.cuda(), ids.cuda(), labels=y.cuda(), teacher_weight=0.0, label_weight=abs(weight), reduction="none")
         assert loss.isinf().tolist() == [False, False, True, False] and loss[2] > 0
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("experts", [8, 17, 200])
+def test_router_logits_of_the_largest_and_lowest_values(experts, dtype):
+    """The gradient of logsumexp^2 there is large, where it is not 0; experts without probability have none of it."""
+    import losses_ref as ref
+
+    least, most = torch.finfo(dtype).min, torch.finfo(dtype).max
+    for fill, at in ((least, None), (least, 0.0), (0.0, least), (0.0, most), (least, most), (0.0, most / 4)):
+        for tokens in (1, 2):
+            r = torch.full((tokens, experts), fill, dtype=dtype)
+            if at is not None:
+                r[0, 3] = at
+            ids = torch.arange(tokens).view(tokens, 1)
+            for up in (0.125, 1e-3):
+                leaf = r.cuda().requires_grad_(True)
+                loss, _ = F.balance_loss(leaf, ids.cuda(), weight=0.5, z_weight=1.0)
+                loss.backward(torch.full((), up, device="cuda"))
+                want, bound, _, grad, gbound = ref.balance(r, ids, None, 0.5, 1.0, float(torch.tensor(up)))
+                what = f"{tokens} x {experts} of {fill} with {at}, factor {up}"
+                ref.assert_within(loss, want, bound, what)
+                ref.assert_within(leaf.grad, grad, gbound, what)
