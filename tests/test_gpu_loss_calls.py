@@ -270,3 +270,34 @@ def test_router_logits_of_the_largest_and_lowest_values(experts, dtype):
                 what = f"{tokens} x {experts} of {fill} with {at}, factor {up}"
                 ref.assert_within(loss, want, bound, what)
                 ref.assert_within(leaf.grad, grad, gbound, what)
+
+
+@pytest.mark.parametrize("make", BOTH)
+def test_threads_with_graphs_of_their_own_and_with_one(make):
+    import threading
+
+    x, loss = make()
+    shared = loss()
+    want = torch.autograd.grad(shared, x, retain_graph=True)[0].clone()
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work():
+        try:
+            stream = torch.cuda.Stream()
+            with torch.cuda.stream(stream):
+                for _ in range(20):
+                    for value in (loss(), shared):
+                        grad = torch.autograd.grad(value, x, retain_graph=value is shared)[0]
+                        torch.cuda.synchronize()
+                        if not torch.equal(grad, want):
+                            wrong.append("gradient")
+        except Exception as e:
+            wrong.append(repr(e))
+
+    threads = [threading.Thread(target=work) for _ in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong, wrong[:3]

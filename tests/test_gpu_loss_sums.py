@@ -169,3 +169,18 @@ def test_rows_of_millions_of_values(dtype, temperature):
     for at, v in ((vocab // 3, low), (100, 0.0)):
         q = temperature * torch.exp(torch.tensor(v / temperature).double()) / sums[0] + 0.5 * torch.exp(torch.tensor(v).double()) / sums[1]
         ref.assert_within(grad[0, at], q, q * (off + U * (3 * -low / min(temperature, 1.0) + 10)), f"gradient of {v}")
+
+
+def test_router_logits_past_32_bits():
+    """The last of 9 million tokens of 256 experts lie past 2^31 values; alone they are what they are behind masked ones."""
+    tokens, experts, last = 9_000_000, 256, 1000
+    r = torch.empty(tokens, experts, device="cuda", dtype=torch.bfloat16).normal_().requires_grad_(True)
+    ids = torch.randint(0, experts, (tokens, 2), device="cuda", dtype=torch.int32)
+    mask = torch.zeros(tokens, dtype=torch.bool, device="cuda")
+    mask[-last:] = True
+    loss, counts = F.balance_loss(r, ids, mask=mask, z_weight=0.1)
+    grad = torch.autograd.grad(loss, r)[0]
+    alone = r.detach()[-last:].clone().requires_grad_(True)
+    want, wcounts = F.balance_loss(alone, ids[-last:], z_weight=0.1)
+    assert torch.equal(counts, wcounts) and abs(float(loss.detach()) - float(want.detach())) <= 4 * U * float(want.detach())
+    assert torch.equal(grad[-last:], torch.autograd.grad(want, alone)[0]) and not grad[:-last].any()
