@@ -104,7 +104,7 @@ void require_seen(const Tensor &t, const char *name, const char *what)
     REQUIRE(!t._fw_grad(0).defined(), name, " has a forward-mode gradient, and ", what, " has no forward-mode derivative");
 }
 
-// Not so of tensors that wrap others: their address is NULL, which for labels and masks would read as none.
+// Whether there is an address to hand to the kernels.  Tensors that wrap others have NULL, which for labels and masks would read as none.
 bool has_memory(const Tensor &t) { return t.numel() == 0 || t.const_data_ptr(); }
 
 struct Named {
